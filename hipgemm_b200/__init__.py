@@ -11,6 +11,9 @@ GEMM:        fp8_gemm_tn (per-tensor scales), fp8_gemm_tn_rows (one rank's rows)
 Quantisers:  quantize_e4m3 (amax/448, two passes), quantize_e4m3_delayed (carried-over
              scale, one pass), quantize_mx_e4m3 (e8m0 per 32 elements, blocked scales),
              mx_sf_to_blocked (host conversion of row-major scales).
+4-bit weights: quantize_w4 / dequantize_w4 (W4Weight: codes with group scales), w4_pack (codes
+             made elsewhere), w4_gemm_tn (a few rows times such a weight), moe_route and w4_moe
+             (a mixture-of-experts layer for a few tokens).
 Host inputs: host_init_random, host_make_quantized (the reference harness's generator).
 Status:      device_status (a kernel's bounded wait expired), HgemmError on negative codes.
 """
@@ -21,6 +24,7 @@ from ._lib import (HGEMM_ERR_ALIGNMENT, HGEMM_ERR_CUDA, HGEMM_ERR_DEVICE_TIMEOUT
 from .gemm import (device_status, fp8_gemm_tn, fp8_gemm_tn_from_host, fp8_gemm_tn_mx, fp8_gemm_tn_rows,
                    host_init_random, host_make_quantized, mx_sf_to_blocked, plan, quantize_e4m3,
                    quantize_e4m3_delayed, quantize_mx_e4m3)
+from .w4 import W4Weight, dequantize_w4, moe_route, quantize_w4, w4_gemm_tn, w4_moe, w4_pack
 
 __all__ = [
     "HGEMM_OK", "HGEMM_ERR_INVALID_VALUE", "HGEMM_ERR_ALIGNMENT", "HGEMM_ERR_UNSUPPORTED", "HGEMM_ERR_CUDA",
@@ -29,4 +33,5 @@ __all__ = [
     "device_status", "fp8_gemm_tn", "fp8_gemm_tn_from_host", "fp8_gemm_tn_mx", "fp8_gemm_tn_rows",
     "host_init_random", "host_make_quantized", "mx_sf_to_blocked", "plan", "quantize_e4m3", "quantize_e4m3_delayed",
     "quantize_mx_e4m3",
+    "W4Weight", "dequantize_w4", "moe_route", "quantize_w4", "w4_gemm_tn", "w4_moe", "w4_pack",
 ]

@@ -66,6 +66,15 @@ _SIGNATURES = {
     "hgemm_mx_config_name": (ctypes.c_char_p, [_i]),
     "hgemm_mx_sf_bytes": (ctypes.c_size_t, [_i, _i]),
     "hgemm_host_mx_sf_to_blocked": (_i, [_vp, _i, _i, _vp]),
+    "hgemm_w4_q_bytes": (ctypes.c_size_t, [_i, _i]),
+    "hgemm_w4_scales": (ctypes.c_size_t, [_i, _i, _i]),
+    "hgemm_quantize_w4": (_i, [_vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
+    "hgemm_dequantize_w4": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _i, _vp]),
+    "hgemm_w4_gemm_tn": (_i, [_vp, _i, ctypes.c_longlong, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "hgemm_moe_route": (_i, [_vp, _i, ctypes.c_longlong, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp]),
+    "hgemm_w4_moe": (_i, [_vp, _i, ctypes.c_longlong, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp,
+                          ctypes.c_size_t, _vp]),
+    "hgemm_w4_moe_workspace_bytes": (ctypes.c_size_t, [_i, _i, _i]),
     "hgemm_num_configs": (_i, []),
     "hgemm_config_resident_ctas": (_i, [_i]),
     "hgemm_config_name": (ctypes.c_char_p, [_i]),

@@ -23,6 +23,7 @@ NVCC_FLAGS = [
     "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC,-O3",
     "--expt-relaxed-constexpr",
+    "--threads", "0",  # the source files in parallel
     "-shared",
 ]
 

@@ -1,0 +1,628 @@
+// A mixture-of-experts layer for a few tokens: the router, and the experts' gated products over
+// 4-bit weights.
+//
+//   route:   logits = x . R^T, p = softmax(logits) over all E experts, the top_k largest
+//   experts: out[t] = sum_j weight[t][j] * down_e( silu(gate_e x[t]) * (up_e x[t]) ),  e = ids[t][j]
+//
+// Both products of the experts read each reached expert's codes once for all the tokens that are
+// sent to it: (token, expert) pairs are grouped by expert into segments of up to 8 NT columns.
+#include <cooperative_groups.h>
+
+#include <atomic>
+
+#include "hipgemm_b200.h"
+#include "w4.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace hgw {
+
+constexpr int kMoeWarps = 8;
+constexpr int kMoeThreads = kMoeWarps * 32;
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxTopK = 16;
+constexpr int kMaxPairs = 512;   // (token, expert) pairs of one launch
+constexpr int kMaxTokens = 64;   // tokens of one launch
+constexpr int kMaxSegments = kMaxPairs;
+
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// ---- router -----------------------------------------------------------------------------
+//
+// A cluster of 8 CTAs takes kRouteTokens tokens; its 64 warps split the experts, each warp a dot
+// product over D for all of the cluster's tokens.  Eight fp32 products a lane are summed in fp32
+// and then added in 64 bits, so that experts whose logits are close are ordered as the exact
+// logits are.  The logits go to the CTA that selects the token's experts over distributed shared
+// memory.
+
+constexpr int kRouteTokens = 4;
+constexpr int kRouteCluster = 8;
+
+struct RouteParams {
+    const void* x;
+    const void* router;
+    long long ldx;
+    int T, D, E, top_k;
+    bool renormalize, vec;
+    int* ids;
+    float* weights;
+};
+
+template <typename T>
+__device__ __forceinline__ void route_load8(const T* row, int at, int len, bool vec, float (&v)[8]) {
+    if (vec) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(row + at));
+            const float4 b = __ldg(reinterpret_cast<const float4*>(row + at) + 1);
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        } else {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + at));
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[2 * i] = bf16_lo(w[i]), v[2 * i + 1] = bf16_hi(w[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (sizeof(T) == 4) v[i] = at + i < len ? row[at + i] : 0.0f;
+            else v[i] = at + i < len ? __bfloat162float(row[at + i]) : 0.0f;
+        }
+    }
+}
+
+// A key that orders as the numbers do, NaN below everything.
+__device__ __forceinline__ unsigned long long order_key(double v) {
+    if (v != v) return 0ull;
+    const unsigned long long b = static_cast<unsigned long long>(__double_as_longlong(v));
+    return b >> 63 ? ~b : b | 0x8000000000000000ull;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kMoeThreads) __cluster_dims__(kRouteCluster, 1, 1) moe_route_kernel(const RouteParams p) {
+    __shared__ double logits[kMaxExperts];  // of the token that this CTA selects for
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = static_cast<int>(cluster.block_rank());
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    const int t0 = static_cast<int>(blockIdx.x) / kRouteCluster * kRouteTokens;
+    pdl_trigger();
+    pdl_wait();
+    cluster.sync();  // every CTA of the cluster runs before its shared memory is written
+
+    const T* x[kRouteTokens];
+#pragma unroll
+    for (int t = 0; t < kRouteTokens; ++t) x[t] = static_cast<const T*>(p.x) + min(t0 + t, p.T - 1) * p.ldx;
+    for (int e = rank * kMoeWarps + warp; e < p.E; e += kRouteCluster * kMoeWarps) {
+        const T* r = static_cast<const T*>(p.router) + static_cast<size_t>(e) * p.D;
+        double sum[kRouteTokens] = {};
+        for (int d = lane * 8; d < p.D; d += 256) {
+            float w[8];
+            route_load8<T>(r, d, p.D, p.vec, w);
+#pragma unroll
+            for (int t = 0; t < kRouteTokens; ++t) {
+                float v[8], s = 0.0f;
+                route_load8<T>(x[t], d, p.D, p.vec, v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s = fmaf(w[i], v[i], s);
+                sum[t] += static_cast<double>(s);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < kRouteTokens; ++t) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum[t] += __shfl_xor_sync(0xffffffffu, sum[t], o);
+        }
+        // Token t of the cluster is selected by CTA t.
+#pragma unroll
+        for (int t = 0; t < kRouteTokens; ++t)
+            if (lane == t) *cluster.map_shared_rank(&logits[e], t) = sum[t];
+    }
+    cluster.sync();
+    // One warp per token: softmax sums, then top_k rounds of a maximum over the keys.
+    const int t = t0 + rank;
+    if (rank >= kRouteTokens || t >= p.T || warp != 0) return;
+    const double* l = logits;
+    double top = -INFINITY;
+    for (int e = lane; e < p.E; e += 32) top = fmax(top, l[e]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float total = 0.0f;
+    for (int e = lane; e < p.E; e += 32) total += expf(static_cast<float>(l[e] - top));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    float mine = 0.0f, chosen = 0.0f;
+    int my_id = 0;
+    unsigned long long taken = 0;  // this lane's experts that are chosen already, by e / 32
+    for (int k = 0; k < p.top_k; ++k) {
+        unsigned long long best = 0;
+        int at = p.E;
+        for (int e = lane, i = 0; e < p.E; e += 32, ++i) {
+            const unsigned long long key = order_key(l[e]);
+            if (!(taken >> i & 1) && (at == p.E || key > best)) best = key, at = e;
+        }
+        int from = at;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
+            const int oe = __shfl_xor_sync(0xffffffffu, from, o);
+            if (oe < p.E && (from == p.E || other > best || (other == best && oe < from))) best = other, from = oe;
+        }
+        if (from == at && at < p.E) taken |= 1ull << (at / 32);
+        const float w = expf(static_cast<float>(l[from] - top)) / total;
+        chosen += w;
+        if (lane == k) mine = w, my_id = from;
+    }
+    if (lane < p.top_k) {
+        const size_t at = static_cast<size_t>(t) * p.top_k + lane;
+        p.ids[at] = my_id;
+        p.weights[at] = p.renormalize ? mine / chosen : mine;
+    }
+}
+
+// ---- grouping pairs by expert ------------------------------------------------------------
+
+struct Segment {
+    short expert, first, columns, unused;  // pairs order[first .. first + columns)
+};
+
+struct PairLists {
+    int count[kMaxExperts];      // pairs of an expert, then its first place in `order`
+    short rank[kMaxPairs];       // a pair's place among its expert's, -1 if it does not count
+    short order[kMaxPairs];      // pairs by expert
+    Segment segments[kMaxSegments];
+    int n_segments;
+};
+
+// Fills the lists from ids (T x top_k), T * top_k <= kMaxPairs.  A pair counts when its id is in
+// [0, E) and its token does not have the same id at an earlier place (the weights of such pairs
+// are added to the first one's).  Within an expert pairs keep their order, so that the sums'
+// order, and with it every bit of the result, depends on the inputs alone.  All threads call it.
+__device__ void build_lists(PairLists& s, const int* ids, int T, int top_k, int E, int columns) {
+    const int pairs = T * top_k;
+    for (int e = threadIdx.x; e < E; e += kMoeThreads) s.count[e] = 0;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x;
+        for (int p0 = 0; p0 < pairs; p0 += 32) {
+            const int p = p0 + lane;
+            int id = -1;
+            if (p < pairs) {
+                id = ids[p];
+                if (id < 0 || id >= E) id = -1;
+                for (int q = p / top_k * top_k; q < p && id >= 0; ++q)
+                    if (ids[q] == id) id = -1;
+            }
+            const unsigned same = __match_any_sync(0xffffffffu, id);
+            const int before = __popc(same & ((1u << lane) - 1u)), base = id >= 0 ? s.count[id] : 0;
+            __syncwarp();
+            if (p < pairs) s.rank[p] = static_cast<short>(id >= 0 ? base + before : -1);
+            if (id >= 0 && before == 0) s.count[id] = base + __popc(same);
+            __syncwarp();
+        }
+        // First places and segments, by a scan over the experts.
+        int pair_at = 0, seg_at = 0;
+        for (int e0 = 0; e0 < E; e0 += 32) {
+            const int e = e0 + lane, n = e < E ? s.count[e] : 0, segs = (n + columns - 1) / columns;
+            int a = n, b = segs;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int ua = __shfl_up_sync(0xffffffffu, a, o), ub = __shfl_up_sync(0xffffffffu, b, o);
+                if (lane >= o) a += ua, b += ub;
+            }
+            const int first = pair_at + a - n;
+            if (e < E) s.count[e] = first;
+            for (int i = 0; i < segs; ++i)
+                s.segments[seg_at + b - segs + i] = {static_cast<short>(e), static_cast<short>(first + i * columns),
+                                                     static_cast<short>(min(columns, n - i * columns)), 0};
+            pair_at += __shfl_sync(0xffffffffu, a, 31);
+            seg_at += __shfl_sync(0xffffffffu, b, 31);
+        }
+        if (lane == 0) s.n_segments = seg_at;
+    }
+    __syncthreads();
+    for (int p = threadIdx.x; p < pairs; p += kMoeThreads)
+        if (s.rank[p] >= 0) s.order[s.count[ids[p]] + s.rank[p]] = static_cast<short>(p);
+    __syncthreads();
+}
+
+// ---- experts: h = silu(gate x) * (up x) ------------------------------------------------------
+//
+// A persistent grid over (segment, RH row blocks of F); the CTA's warps split D.  h is kept as
+// two bf16 whose sum has 16 significant bits or more: twice the matrix instructions in the
+// product with down, which the codes' bandwidth hides, and no rounding to 8 bits between the
+// two products.
+
+struct ExpertParams {
+    const void* x;
+    long long ldx;
+    const int* ids;
+    const float* weights;
+    int T, top_k, E, D, F;
+    Weight gate, up, down;
+    bool vec;
+    __nv_bfloat16* h;       // [2][kMaxPairs rows used][h_stride]
+    int h_stride;           // row blocks of F, in elements
+    long long h_low;        // elements from the upper part to the lower one
+    void* out;
+};
+
+template <typename T, int RH, int NT, int DEPTH, bool G32, bool ZERO>
+__global__ void __launch_bounds__(kMoeThreads) moe_gate_up_kernel(const ExpertParams p) {
+    constexpr int kOut = 2 * RH * NT * 128;
+    __shared__ PairLists lists;
+    __shared__ float partial[kMoeWarps][kOut];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    pdl_trigger();
+    pdl_wait();
+    build_lists(lists, p.ids, p.T, p.top_k, p.E, 8 * NT);
+    const int chunks = (p.gate.row_blocks + RH - 1) / RH, units = lists.n_segments * chunks;
+    const int kb0 = p.gate.k_blocks * warp / kMoeWarps, kb1 = p.gate.k_blocks * (warp + 1) / kMoeWarps;
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+        const int seg = u / chunks, block0 = (u - seg * chunks) * RH;
+        const Segment sg = lists.segments[seg];
+        WarpProduct<2 * RH, NT, DEPTH, G32, ZERO, RowSource<T>> product;
+#pragma unroll
+        for (int r = 0; r < RH; ++r) {
+            const int block = min(block0 + r, p.gate.row_blocks - 1);
+            product.set_rows(r, p.gate, sg.expert, block, lane);
+            product.set_rows(RH + r, p.up, sg.expert, block, lane);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int pair = lists.order[sg.first + min(8 * n + lane / 4, sg.columns - 1)];
+            product.x[n] = {static_cast<const T*>(p.x) + static_cast<long long>(pair / p.top_k) * p.ldx, p.D, p.vec};
+        }
+        float acc[2 * RH][NT][4] = {};
+        product.run(kb0, kb1, lane, acc);
+#pragma unroll
+        for (int r = 0; r < 2 * RH; ++r)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) partial[warp][((r * NT + n) * 4 + i) * 32 + lane] = acc[r][n][i];
+        __syncthreads();
+        for (int i = threadIdx.x; i < kOut / 2; i += kMoeThreads) {
+            float g = 0.0f, v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kMoeWarps; ++w) {
+                g += partial[w][i];
+                v += partial[w][kOut / 2 + i];
+            }
+            const int l = i & 31, f = (i >> 5) & 3, n = (i >> 7) % NT, r = (i >> 7) / NT;
+            const int row = (block0 + r) * 16 + l / 4 + 8 * (f >> 1), col = 8 * n + 2 * (l & 3) + (f & 1);
+            if (row < p.h_stride && col < sg.columns) {
+                // Rows past F (up to the row block's end) are zeros, which the next product may read.
+                const float h = row < p.F ? g / (1.0f + expf(-g)) * v : 0.0f;
+                const float low = after_bf16(h);
+                const size_t at = static_cast<size_t>(lists.order[sg.first + col]) * p.h_stride + row;
+                p.h[at] = __ushort_as_bfloat16(static_cast<unsigned short>(__float_as_uint(h) >> 16));
+                p.h[at + p.h_low] = __float2bfloat16_rn(low);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---- experts: out = sum of the weighted products with down -------------------------------------
+//
+// A cluster takes R row blocks of D for all pairs: the list of (segment, K block) steps is split
+// over its warps, and each warp adds its part of a segment, times the router's weight, to its own
+// sums of every token.  The warps' sums, then the CTAs', are joined in a fixed order.
+
+// Rows of h: two bf16 terms, 16-byte aligned, a multiple of 16 long.
+struct SplitSource {
+    static constexpr int kTerms = 2;
+    struct Raw {
+        uint4 v[4];
+    };
+    const __nv_bfloat16* row;
+    long long low;
+    int len;
+    __device__ __forceinline__ void load(Raw& raw, int k) const {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int at = k + 32 * h;
+            raw.v[h] = raw.v[2 + h] = make_uint4(0u, 0u, 0u, 0u);
+            if (at < len) {
+                raw.v[h] = *reinterpret_cast<const uint4*>(row + at);
+                raw.v[2 + h] = *reinterpret_cast<const uint4*>(row + low + at);
+            }
+        }
+    }
+    __device__ __forceinline__ static void terms(const Raw& raw, uint32_t (&b)[2][8]) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                b[s][4 * h] = raw.v[2 * s + h].x;
+                b[s][4 * h + 1] = raw.v[2 * s + h].y;
+                b[s][4 * h + 2] = raw.v[2 * s + h].z;
+                b[s][4 * h + 3] = raw.v[2 * s + h].w;
+            }
+    }
+};
+
+template <int R>
+struct DownShape {
+    static constexpr int kRows = 16 * R;
+    static constexpr int kStride = kRows + 8;  // a token's sums: columns 2 t, 2 t + 1 of a warp's store to distinct banks
+    static size_t smem(int tokens) { return static_cast<size_t>(kMoeWarps) * tokens * kStride * sizeof(float); }
+};
+
+template <typename T, int R, int NT, int DEPTH, bool G32, bool ZERO>
+__global__ void __launch_bounds__(kMoeThreads) moe_down_kernel(const ExpertParams p) {
+    using Shape = DownShape<R>;
+    extern __shared__ float sums[];  // [warp][token][kStride]
+    __shared__ PairLists lists;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int split = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    const int block0 = static_cast<int>(blockIdx.x) / split * R;
+    pdl_trigger();
+    pdl_wait();
+    const int per_warp = p.T * Shape::kStride;
+    for (int i = threadIdx.x; i < kMoeWarps * per_warp; i += kMoeThreads) sums[i] = 0.0f;
+    build_lists(lists, p.ids, p.T, p.top_k, p.E, 8 * NT);
+
+    float* mine = sums + warp * per_warp;
+    const int k_blocks = p.down.k_blocks, parts = split * kMoeWarps, part = rank * kMoeWarps + warp;
+    const long long steps = static_cast<long long>(lists.n_segments) * k_blocks;
+    long long step = steps * part / parts;
+    const long long end = steps * (part + 1) / parts;
+    while (step < end) {
+        const int seg = static_cast<int>(step / k_blocks), kb0 = static_cast<int>(step - static_cast<long long>(seg) * k_blocks);
+        const int kb1 = static_cast<int>(min(static_cast<long long>(k_blocks), kb0 + (end - step)));
+        step += kb1 - kb0;
+        const Segment sg = lists.segments[seg];
+        WarpProduct<R, NT, DEPTH, G32, ZERO, SplitSource> product;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            product.set_rows(r, p.down, sg.expert, min(block0 + r, p.down.row_blocks - 1), lane);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int pair = lists.order[sg.first + min(8 * n + lane / 4, sg.columns - 1)];
+            product.x[n] = {p.h + static_cast<size_t>(pair) * p.h_stride, p.h_low, p.h_stride};
+        }
+        float acc[R][NT][4] = {};
+        product.run(kb0, kb1, lane, acc);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int col = 8 * n + 2 * (lane & 3) + c;
+                if (col >= sg.columns) continue;
+                const int pair = lists.order[sg.first + col], token = pair / p.top_k;
+                float weight = 0.0f;
+                for (int j = pair; j < (token + 1) * p.top_k; ++j)
+                    if (j == pair || p.ids[j] == sg.expert) weight += p.weights[j];
+                // A segment's columns are distinct tokens: no two lanes add to the same sum.
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        float* at = mine + token * Shape::kStride + 16 * r + lane / 4 + 8 * half;
+                        *at = fmaf(weight, acc[r][n][2 * half + c], *at);
+                    }
+            }
+        __syncwarp();
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < per_warp; i += kMoeThreads) {
+        float v = sums[i];
+#pragma unroll
+        for (int w = 1; w < kMoeWarps; ++w) v += sums[w * per_warp + i];
+        sums[i] = v;
+    }
+    cluster.sync();
+    const int outputs = p.T * Shape::kRows;
+    for (int i = rank * kMoeThreads + threadIdx.x; i < outputs; i += split * kMoeThreads) {
+        const int token = i / Shape::kRows, r = i - token * Shape::kRows, row = block0 * 16 + r;
+        float v = 0.0f;
+        for (int s = 0; s < split; ++s) v += cluster.map_shared_rank(sums, s)[token * Shape::kStride + r];
+        if (row < p.D) {
+            T* dst = static_cast<T*>(p.out) + static_cast<size_t>(token) * p.D + row;
+            if constexpr (sizeof(T) == 4) *dst = v;
+            else *dst = __float2bfloat16_rn(v);
+        }
+    }
+    cluster.sync();  // no CTA leaves while another reads its sums
+}
+
+// ---- host -----------------------------------------------------------------------------------
+
+inline int tokens_per_launch(int top_k) {
+    const int t = kMaxPairs / top_k;
+    return t < kMaxTokens ? t : kMaxTokens;
+}
+
+template <typename Kernel>
+int launch(Kernel kernel, unsigned grid, unsigned cluster, size_t smem, cudaStream_t stream, const ExpertParams& p) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid, 1, 1);
+    cfg.blockDim = dim3(kMoeThreads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    if (cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess) return HGEMM_OK;
+    cudaGetLastError();
+    return HGEMM_ERR_CUDA;
+}
+
+template <typename T, int RH, int NT, int DEPTH, bool G32, bool ZERO>
+int launch_gate_up(const ExpertParams& p, int sms, cudaStream_t stream) {
+    auto kernel = moe_gate_up_kernel<T, RH, NT, DEPTH, G32, ZERO>;
+    static std::atomic<int> per_sm{0};  // the same on every sm_100 device
+    int b = per_sm.load(std::memory_order_relaxed);
+    if (b == 0) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&b, kernel, kMoeThreads, 0) != cudaSuccess || b < 1) b = 1;
+        per_sm.store(b, std::memory_order_relaxed);
+    }
+    const int pairs = p.T * p.top_k, experts = pairs < p.E ? pairs : p.E;
+    const long long most = static_cast<long long>(experts + pairs / (8 * NT)) * ceil_div(p.gate.row_blocks, RH);
+    const long long wave = static_cast<long long>(sms) * b;
+    return launch(kernel, static_cast<unsigned>(most < wave ? most : wave), 1, 0, stream, p);
+}
+
+template <typename T, int R, int NT, int DEPTH, bool G32, bool ZERO>
+int launch_down(const ExpertParams& p, int sms, cudaStream_t stream) {
+    auto kernel = moe_down_kernel<T, R, NT, DEPTH, G32, ZERO>;
+    const size_t smem = DownShape<R>::smem(p.T);
+    static std::atomic<unsigned long long> ready{0};  // per device: the kernel may have its largest shared memory
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return HGEMM_ERR_NO_DEVICE;
+    if (!(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(DownShape<R>::smem(kMaxTokens))) != cudaSuccess) {
+            cudaGetLastError();
+            return HGEMM_ERR_CUDA;
+        }
+        ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
+    const int groups = ceil_div(p.down.row_blocks, R);
+    int split = 1;
+    while (split < 8 && groups * split < 2 * sms) split *= 2;
+    return launch(kernel, static_cast<unsigned>(groups) * split, static_cast<unsigned>(split), smem, stream, p);
+}
+
+template <typename T, bool G32, bool ZERO>
+int run_gate_up(const ExpertParams& p, int sms, cudaStream_t stream) {
+    if constexpr (sizeof(T) == 4) {
+        return launch_gate_up<T, 1, 1, 2, G32, ZERO>(p, sms, stream);
+    } else {
+        if (p.T * p.top_k <= 8 * p.E) return launch_gate_up<T, 1, 1, 4, G32, ZERO>(p, sms, stream);
+        return launch_gate_up<T, 1, 2, 2, G32, ZERO>(p, sms, stream);
+    }
+}
+
+template <typename T, bool G32, bool ZERO>
+int run_down(const ExpertParams& p, int sms, cudaStream_t stream) {
+    return launch_down<T, 2, 1, 2, G32, ZERO>(p, sms, stream);
+}
+
+inline bool misaligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1u)) != 0; }
+
+inline size_t h_stride(int F) { return static_cast<size_t>(ceil_div(F, kTileRows)) * kTileRows; }
+
+}  // namespace hgw
+
+extern "C" {
+
+int hgemm_moe_route(const void* x, int x_dtype, long long ldx, const void* router, int T, int D, int E, int top_k,
+                    int renormalize, int* ids, float* weights, hgemm_stream_t stream) {
+    if (T < 0 || D < 0 || E < 1 || top_k < 1 || top_k > E) return HGEMM_ERR_INVALID_VALUE;
+    if (x_dtype != HGEMM_DTYPE_F32 && x_dtype != HGEMM_DTYPE_BF16) return HGEMM_ERR_INVALID_VALUE;
+    if (E > hgw::kMaxExperts || top_k > hgw::kMaxTopK) return HGEMM_ERR_UNSUPPORTED;
+    if (T > 1 && ldx < D) return HGEMM_ERR_INVALID_VALUE;
+    if (T == 0) return HGEMM_OK;
+    if (!ids || !weights || (D > 0 && (!x || !router))) return HGEMM_ERR_INVALID_VALUE;
+    const unsigned size = x_dtype == HGEMM_DTYPE_F32 ? 4 : 2;
+    if (hgw::misaligned(x, size) || hgw::misaligned(router, size) || hgw::misaligned(ids, 4) || hgw::misaligned(weights, 4))
+        return HGEMM_ERR_ALIGNMENT;
+    int sms = 0;
+    if (int rc = hgw::current_sms(&sms)) return rc;
+    hgw::RouteParams p{x, router, T > 1 ? ldx : 0, T, D, E, top_k, renormalize != 0, false, ids, weights};
+    p.vec = !hgw::misaligned(x, 16) && !hgw::misaligned(router, 16) && D % 8 == 0 && p.ldx % (16 / size) == 0;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(hgw::ceil_div(T, hgw::kRouteTokens)) * hgw::kRouteCluster, 1, 1);
+    cfg.blockDim = dim3(hgw::kMoeThreads, 1, 1);
+    cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = x_dtype == HGEMM_DTYPE_F32 ? cudaLaunchKernelEx(&cfg, hgw::moe_route_kernel<float>, p)
+                                                     : cudaLaunchKernelEx(&cfg, hgw::moe_route_kernel<__nv_bfloat16>, p);
+    if (e == cudaSuccess) return HGEMM_OK;
+    cudaGetLastError();
+    return HGEMM_ERR_CUDA;
+}
+
+size_t hgemm_w4_moe_workspace_bytes(int T, int top_k, int F) {
+    if (T <= 0 || top_k <= 0 || top_k > hgw::kMaxTopK || F <= 0) return 0;
+    const int most = hgw::tokens_per_launch(top_k), tokens = T < most ? T : most;
+    return static_cast<size_t>(tokens) * top_k * hgw::h_stride(F) * 4;  // two bf16 per element of h
+}
+
+int hgemm_w4_moe(const void* x, int x_dtype, long long ldx, const int* ids, const float* weights, int T, int top_k, int E,
+                 int D, int F, const hgemm_w4_weight* gate, const hgemm_w4_weight* up, const hgemm_w4_weight* down,
+                 void* out, void* workspace, size_t workspace_bytes, hgemm_stream_t stream) {
+    if (T < 0 || D < 0 || F < 0 || E < 1 || top_k < 1 || !gate || !up || !down) return HGEMM_ERR_INVALID_VALUE;
+    if (x_dtype != HGEMM_DTYPE_F32 && x_dtype != HGEMM_DTYPE_BF16) return HGEMM_ERR_INVALID_VALUE;
+    if (!hgw::valid_group(gate->group) || !hgw::valid_group(up->group) || !hgw::valid_group(down->group))
+        return HGEMM_ERR_INVALID_VALUE;
+    if (E > hgw::kMaxExperts || top_k > hgw::kMaxTopK) return HGEMM_ERR_UNSUPPORTED;
+    if (gate->group != up->group || !gate->zeros != !up->zeros) return HGEMM_ERR_UNSUPPORTED;
+    if (T > 1 && ldx < D) return HGEMM_ERR_INVALID_VALUE;
+    if (T == 0 || D == 0) return HGEMM_OK;
+    if (!x || !ids || !weights || !out) return HGEMM_ERR_INVALID_VALUE;
+    const unsigned size = x_dtype == HGEMM_DTYPE_F32 ? 4 : 2;
+    if (hgw::misaligned(x, size) || hgw::misaligned(out, size) || hgw::misaligned(ids, 4) || hgw::misaligned(weights, 4))
+        return HGEMM_ERR_ALIGNMENT;
+    const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    int sms = 0;
+    if (F == 0) {
+        if (int rc = hgw::current_sms(&sms)) return rc;
+        return cudaMemsetAsync(out, 0, static_cast<size_t>(T) * D * size, s) == cudaSuccess ? HGEMM_OK : HGEMM_ERR_CUDA;
+    }
+    for (const hgemm_w4_weight* w : {gate, up, down}) {
+        if (!w->q || !w->scales) return HGEMM_ERR_INVALID_VALUE;
+        if (hgw::misaligned(w->q, 16) || hgw::misaligned(w->scales, 4) || hgw::misaligned(w->zeros, 2))
+            return HGEMM_ERR_ALIGNMENT;
+    }
+    if (!workspace || workspace_bytes < hgemm_w4_moe_workspace_bytes(T, top_k, F)) return HGEMM_ERR_INVALID_VALUE;
+    if (hgw::misaligned(workspace, 16)) return HGEMM_ERR_ALIGNMENT;
+    if (int rc = hgw::current_sms(&sms)) return rc;
+
+    const int most = hgw::tokens_per_launch(top_k);
+    hgw::ExpertParams p{};
+    p.ldx = T > 1 ? ldx : 0;
+    p.top_k = top_k;
+    p.E = E;
+    p.D = D;
+    p.F = F;
+    p.gate = hgw::make_weight(gate->q, gate->scales, gate->zeros, F, D, gate->group);
+    p.up = hgw::make_weight(up->q, up->scales, up->zeros, F, D, up->group);
+    p.down = hgw::make_weight(down->q, down->scales, down->zeros, D, F, down->group);
+    p.vec = !hgw::misaligned(x, 16) && D % 8 == 0 && p.ldx % (16 / size) == 0;
+    p.h = static_cast<__nv_bfloat16*>(workspace);
+    p.h_stride = static_cast<int>(hgw::h_stride(F));
+    p.h_low = static_cast<long long>(T < most ? T : most) * top_k * p.h_stride;
+    using True = std::true_type;
+    using False = std::false_type;
+    auto pick = [](const hgemm_w4_weight* w, auto go) {
+        if (w->group == 32) return w->zeros ? go(True{}, True{}) : go(True{}, False{});
+        return w->zeros ? go(False{}, True{}) : go(False{}, False{});
+    };
+    // Launches of up to kMaxTokens tokens; they share the workspace, in stream order.
+    for (int t0 = 0; t0 < T; t0 += most) {
+        p.T = T - t0 < most ? T - t0 : most;
+        p.x = static_cast<const char*>(x) + static_cast<size_t>(t0) * ldx * size;
+        p.ids = ids + static_cast<size_t>(t0) * top_k;
+        p.weights = weights + static_cast<size_t>(t0) * top_k;
+        p.out = static_cast<char*>(out) + static_cast<size_t>(t0) * D * size;
+        int rc = pick(gate, [&](auto g, auto z) {
+            constexpr bool G = decltype(g)::value, Z = decltype(z)::value;
+            return x_dtype == HGEMM_DTYPE_F32 ? hgw::run_gate_up<float, G, Z>(p, sms, s)
+                                              : hgw::run_gate_up<__nv_bfloat16, G, Z>(p, sms, s);
+        });
+        if (rc) return rc;
+        rc = pick(down, [&](auto g, auto z) {
+            constexpr bool G = decltype(g)::value, Z = decltype(z)::value;
+            return x_dtype == HGEMM_DTYPE_F32 ? hgw::run_down<float, G, Z>(p, sms, s)
+                                              : hgw::run_down<__nv_bfloat16, G, Z>(p, sms, s);
+        });
+        if (rc) return rc;
+    }
+    return HGEMM_OK;
+}
+
+}  // extern "C"

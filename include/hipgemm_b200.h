@@ -271,6 +271,79 @@ int hgemm_quantize_e4m3_delayed(const void* x, int x_dtype, size_t n, void* q, c
 int hgemm_quantize_mx_e4m3(const void* x, int x_dtype, int rows, int K, void* q, void* sf_blocked,
                            hgemm_stream_t stream);
 
+/* ---- 4-bit weights with group scales ------------------------------------------------------ */
+
+/* W[n][k] = (code[n][k] - zero) * scale: codes 0..15, one bf16 scale per row and `group`
+ * consecutive K (32, 64 or 128; the last group of a row may be shorter) and, if asymmetric,
+ * one zero point 0..15 (else 8).  Any N and K.  Buffers:
+ *   q       hgemm_w4_q_bytes(N, K) bytes, 16-byte aligned: blocks of 16 rows x 64 K, 512 bytes each,
+ *           [row block][K block]; byte 16 (4 g + t) + 4 (2 jg + jk) + 2 half + rk of a block holds
+ *           the codes of k = 32 jg + 8 t + 4 jk + 2 rk + half in row g (low nibble) and row g + 8
+ *           (high nibble), g = 0..7, t = 0..3, the others 0..1.  Padding may hold anything.
+ *   scales  hgemm_w4_scales(N, K, group) bf16, 4-byte aligned: [row block][group][g][2], rows g
+ *           and g + 8 of the block.
+ *   zeros   as many bytes in the same order, 2-byte aligned, or NULL.
+ * A stack of `count` matrices (experts) is their buffers back to back. */
+size_t hgemm_w4_q_bytes(int N, int K);
+size_t hgemm_w4_scales(int N, int K, int group);
+
+/* w (count x N x K row-major fp32 or bf16) -> q, scales and, where zeros is not NULL, zeros.
+ *   symmetric:  scale = bf16(fp32(amax / 7)), code = clamp(rint(w / scale), -8, 7) + 8
+ *   asymmetric: scale = bf16(fp32((max - min) / 15)), zero = clamp(rint(-min / scale), 0, 15),
+ *               code = clamp(rint(w / scale) + zero, 0, 15), with min <= 0 <= max
+ * per row and group; quotients as exact arithmetic gives them, ties to even, a scale of 0
+ * becomes 1 and one above the largest bf16 that; NaN elements take the code of 0 and do not
+ * count toward the scale.  The padding's codes stand for 0; padding rows have scale 1 and zero
+ * point 0.  Stream-ordered, no sync. */
+int hgemm_quantize_w4(const void* w, int w_dtype, int count, int N, int K, int group, void* q, void* scales, void* zeros,
+                      hgemm_stream_t stream);
+
+/* The inverse: w[n][k] = (code - zero) * scale, exact in fp32 and rounded once to w_dtype. */
+int hgemm_dequantize_w4(const void* q, const void* scales, const void* zeros, int count, int N, int K, int group, void* w,
+                        int w_dtype, hgemm_stream_t stream);
+
+/* y[M x N] = x[M x K] . W[N x K]^T for few rows of x (decoding): x fp32 or bf16 with `ldx`
+ * elements from row to row, y row-major of the same type, sums in fp32, one rounding.  x is used
+ * as it is (fp32 in full).  Any M, N, K; y is fully overwritten; K == 0 writes zeros.  W is read
+ * once per 8 rows of fp32 or 32 rows of bf16 x, so for many rows dequantise it instead.  The
+ * result's bits depend on the inputs alone.  Needs no workspace.  x, y aligned to their element. */
+int hgemm_w4_gemm_tn(const void* x, int x_dtype, long long ldx, const void* q, const void* scales, const void* zeros,
+                     void* y, int M, int N, int K, int group, hgemm_stream_t stream);
+
+/* ---- mixture of experts ----------------------------------------------------------------------- */
+
+/* The router of a mixture of experts: logits = x[T x D] . router[E x D]^T (both of x_dtype),
+ * p = softmax over all E, and per token the top_k largest: ids (T x top_k, largest first, ties to
+ * the lower index, NaN last) and weights (p of those, divided by their sum if renormalize).
+ * E <= 1024 and top_k <= 16, else HGEMM_ERR_UNSUPPORTED.  Needs no workspace. */
+int hgemm_moe_route(const void* x, int x_dtype, long long ldx, const void* router, int T, int D, int E, int top_k,
+                    int renormalize, int* ids, float* weights, hgemm_stream_t stream);
+
+/* A weight as the functions above take it, for calls that take several. */
+typedef struct {
+    const void* q;
+    const void* scales;
+    const void* zeros; /* or NULL */
+    int group;
+} hgemm_w4_weight;
+
+/* The experts of a few tokens, in two kernels:
+ *   out[t] = sum_j weights[t][j] * down_e( silu(gate_e x[t]) * (up_e x[t]) ),  e = ids[t][j].
+ * x: T x D fp32 or bf16, `ldx` elements from row to row; out: T x D row-major of the same type;
+ * gate and up: stacks of E (F x D) of the same group size, both with or both without zero
+ * points; down: a stack of E (D x F).  An id outside [0, E) adds nothing (padding, experts of
+ * another rank); an id that a token has twice counts with both weights.  Sums in fp32; the
+ * product between the two kernels is kept in 16 significant bits or more.  Codes of an expert are
+ * read once per 8 or 16 of its tokens; tokens beyond 64 (or 512 / top_k) take further launches.  The
+ * result's bits depend on the inputs alone.
+ * workspace: device memory, 16-byte aligned, hgemm_w4_moe_workspace_bytes(); its content does not
+ * matter.  Calls that share one must not overlap on the GPU.  E <= 1024 and top_k <= 16, else
+ * HGEMM_ERR_UNSUPPORTED. */
+int hgemm_w4_moe(const void* x, int x_dtype, long long ldx, const int* ids, const float* weights, int T, int top_k, int E,
+                 int D, int F, const hgemm_w4_weight* gate, const hgemm_w4_weight* up, const hgemm_w4_weight* down,
+                 void* out, void* workspace, size_t workspace_bytes, hgemm_stream_t stream);
+size_t hgemm_w4_moe_workspace_bytes(int T, int top_k, int F);
+
 /* ---- host utilities mirroring the reference harness (utils.hpp) ---------------------- */
 
 /* utils.hpp:27-33 init_random, generalised: std::mt19937(seed) feeding
