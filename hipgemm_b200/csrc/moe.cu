@@ -25,9 +25,6 @@ constexpr int kMaxPairs = 512;   // (token, expert) pairs of one launch
 constexpr int kMaxTokens = 64;   // tokens of one launch
 constexpr int kMaxSegments = kMaxPairs;
 
-__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // ---- router -----------------------------------------------------------------------------
 //
 // A cluster of 8 CTAs takes kRouteTokens tokens; its 64 warps split the experts, each warp a dot
@@ -227,10 +224,10 @@ __device__ void build_lists(PairLists& s, const int* ids, int T, int top_k, int 
 
 // ---- experts: h = silu(gate x) * (up x) ------------------------------------------------------
 //
-// A persistent grid over (segment, RH row blocks of F); the CTA's warps split D.  h is kept as
-// two bf16 whose sum has 16 significant bits or more: twice the matrix instructions in the
-// product with down, which the codes' bandwidth hides, and no rounding to 8 bits between the
-// two products.
+// A persistent grid over (segment, RH row blocks of F); the CTA's warps split D.  For bf16 x, h is
+// kept as two bf16 whose sum has 16 significant bits or more: twice the matrix instructions in
+// the product with down, and no rounding to 8 bits between the two products, which would add as
+// much error as the output's own rounding.  For fp32 x it is kept in fp32.
 
 struct ExpertParams {
     const void* x;
@@ -240,27 +237,36 @@ struct ExpertParams {
     int T, top_k, E, D, F;
     Weight gate, up, down;
     bool vec;
-    __nv_bfloat16* h;       // [2][kMaxPairs rows used][h_stride]
-    int h_stride;           // row blocks of F, in elements
-    long long h_low;        // elements from the upper part to the lower one
+    void* h;                // rows of h_stride elements by pair: fp32, or upper bf16 and h_low elements on the lower ones
+    int h_stride;           // F rounded up to whole row blocks
+    long long h_low;
     void* out;
 };
 
-template <typename T, int RH, int NT, int DEPTH, bool G32, bool ZERO>
+template <typename T, int RH, int NT, int STAGES, int GROUP, bool ZERO>
+struct GateUpShape {
+    using Product = WarpProduct<2 * RH, NT, STAGES, GROUP, ZERO, RowSource<T>>;
+    static constexpr int kOut = 2 * RH * NT * 128;
+    static constexpr int kRings = kMoeWarps * Product::kWarpBytes, kSmem = kRings + kMoeWarps * kOut * 4;
+};
+
+template <typename T, int RH, int NT, int STAGES, int GROUP, bool ZERO>
 __global__ void __launch_bounds__(kMoeThreads) moe_gate_up_kernel(const ExpertParams p) {
-    constexpr int kOut = 2 * RH * NT * 128;
+    using Shape = GateUpShape<T, RH, NT, STAGES, GROUP, ZERO>;
+    constexpr int kOut = Shape::kOut;
+    extern __shared__ __align__(16) uint8_t smem[];  // the warps' rings, then their sums
+    float* partial = reinterpret_cast<float*>(smem + Shape::kRings);
     __shared__ PairLists lists;
-    __shared__ float partial[kMoeWarps][kOut];
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     pdl_trigger();
     pdl_wait();
     build_lists(lists, p.ids, p.T, p.top_k, p.E, 8 * NT);
     const int chunks = (p.gate.row_blocks + RH - 1) / RH, units = lists.n_segments * chunks;
-    const int kb0 = p.gate.k_blocks * warp / kMoeWarps, kb1 = p.gate.k_blocks * (warp + 1) / kMoeWarps;
+    const int steps = ceil_div(p.gate.k_blocks, 2), s0 = steps * warp / kMoeWarps, s1 = steps * (warp + 1) / kMoeWarps;
     for (int u = blockIdx.x; u < units; u += gridDim.x) {
         const int seg = u / chunks, block0 = (u - seg * chunks) * RH;
         const Segment sg = lists.segments[seg];
-        WarpProduct<2 * RH, NT, DEPTH, G32, ZERO, RowSource<T>> product;
+        typename Shape::Product product;
 #pragma unroll
         for (int r = 0; r < RH; ++r) {
             const int block = min(block0 + r, p.gate.row_blocks - 1);
@@ -269,34 +275,39 @@ __global__ void __launch_bounds__(kMoeThreads) moe_gate_up_kernel(const ExpertPa
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const int pair = lists.order[sg.first + min(8 * n + lane / 4, sg.columns - 1)];
-            product.x[n] = {static_cast<const T*>(p.x) + static_cast<long long>(pair / p.top_k) * p.ldx, p.D, p.vec};
+            const int pair = lists.order[sg.first + min(8 * n + lane / 4, sg.columns - 1)], k = 8 * (lane & 3);
+            product.x[n] = {static_cast<const T*>(p.x) + static_cast<long long>(pair / p.top_k) * p.ldx + k, p.D - k, p.vec};
         }
+        product.set_columns(p.vec ? p.D : 0);
         float acc[2 * RH][NT][4] = {};
-        product.run(kb0, kb1, lane, acc);
+        product.run(smem + warp * Shape::Product::kWarpBytes, s0, s1, lane, acc);
 #pragma unroll
         for (int r = 0; r < 2 * RH; ++r)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) partial[warp][((r * NT + n) * 4 + i) * 32 + lane] = acc[r][n][i];
+                for (int i = 0; i < 4; ++i) partial[warp * kOut + ((r * NT + n) * 4 + i) * 32 + lane] = acc[r][n][i];
         __syncthreads();
         for (int i = threadIdx.x; i < kOut / 2; i += kMoeThreads) {
             float g = 0.0f, v = 0.0f;
 #pragma unroll
             for (int w = 0; w < kMoeWarps; ++w) {
-                g += partial[w][i];
-                v += partial[w][kOut / 2 + i];
+                g += partial[w * kOut + i];
+                v += partial[w * kOut + kOut / 2 + i];
             }
             const int l = i & 31, f = (i >> 5) & 3, n = (i >> 7) % NT, r = (i >> 7) / NT;
             const int row = (block0 + r) * 16 + l / 4 + 8 * (f >> 1), col = 8 * n + 2 * (l & 3) + (f & 1);
             if (row < p.h_stride && col < sg.columns) {
                 // Rows past F (up to the row block's end) are zeros, which the next product may read.
                 const float h = row < p.F ? g / (1.0f + expf(-g)) * v : 0.0f;
-                const float low = after_bf16(h);
                 const size_t at = static_cast<size_t>(lists.order[sg.first + col]) * p.h_stride + row;
-                p.h[at] = __ushort_as_bfloat16(static_cast<unsigned short>(__float_as_uint(h) >> 16));
-                p.h[at + p.h_low] = __float2bfloat16_rn(low);
+                if constexpr (sizeof(T) == 4) {
+                    static_cast<float*>(p.h)[at] = h;
+                } else {
+                    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.h) + at;
+                    dst[0] = __ushort_as_bfloat16(static_cast<unsigned short>(__float_as_uint(h) >> 16));
+                    dst[p.h_low] = __float2bfloat16_rn(after_bf16(h));
+                }
             }
         }
         __syncthreads();
@@ -309,15 +320,22 @@ __global__ void __launch_bounds__(kMoeThreads) moe_gate_up_kernel(const ExpertPa
 // over its warps, and each warp adds its part of a segment, times the router's weight, to its own
 // sums of every token.  The warps' sums, then the CTAs', are joined in a fixed order.
 
-// Rows of h: two bf16 terms, 16-byte aligned, a multiple of 16 long.
+// Rows of h as two bf16 terms, 16-byte aligned and a multiple of 16 long.
 struct SplitSource {
     static constexpr int kTerms = 2;
     struct Raw {
         uint4 v[4];
     };
     const __nv_bfloat16* row;
-    long long low;
     int len;
+    long long low;
+    __device__ __forceinline__ void load_full(Raw& raw, int k) const {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            raw.v[h] = reinterpret_cast<const uint4*>(row + k)[4 * h];
+            raw.v[2 + h] = reinterpret_cast<const uint4*>(row + low + k)[4 * h];
+        }
+    }
     __device__ __forceinline__ void load(Raw& raw, int k) const {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -342,17 +360,21 @@ struct SplitSource {
     }
 };
 
-template <int R>
+template <typename T, int R, int NT, int STAGES, int GROUP, bool ZERO>
 struct DownShape {
+    using Source = std::conditional_t<sizeof(T) == 4, RowSource<float>, SplitSource>;
+    using Product = WarpProduct<R, NT, STAGES, GROUP, ZERO, Source>;
     static constexpr int kRows = 16 * R;
     static constexpr int kStride = kRows + 8;  // a token's sums: columns 2 t, 2 t + 1 of a warp's store to distinct banks
-    static size_t smem(int tokens) { return static_cast<size_t>(kMoeWarps) * tokens * kStride * sizeof(float); }
+    static constexpr int kRings = kMoeWarps * Product::kWarpBytes;
+    static constexpr int smem(int tokens) { return kRings + kMoeWarps * tokens * kStride * 4; }
 };
 
-template <typename T, int R, int NT, int DEPTH, bool G32, bool ZERO>
+template <typename T, int R, int NT, int STAGES, int GROUP, bool ZERO>
 __global__ void __launch_bounds__(kMoeThreads) moe_down_kernel(const ExpertParams p) {
-    using Shape = DownShape<R>;
-    extern __shared__ float sums[];  // [warp][token][kStride]
+    using Shape = DownShape<T, R, NT, STAGES, GROUP, ZERO>;
+    extern __shared__ __align__(16) uint8_t smem[];
+    float* sums = reinterpret_cast<float*>(smem + Shape::kRings);  // [warp][token][kStride]
     __shared__ PairLists lists;
     cg::cluster_group cluster = cg::this_cluster();
     const int split = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
@@ -365,26 +387,29 @@ __global__ void __launch_bounds__(kMoeThreads) moe_down_kernel(const ExpertParam
     build_lists(lists, p.ids, p.T, p.top_k, p.E, 8 * NT);
 
     float* mine = sums + warp * per_warp;
-    const int k_blocks = p.down.k_blocks, parts = split * kMoeWarps, part = rank * kMoeWarps + warp;
-    const long long steps = static_cast<long long>(lists.n_segments) * k_blocks;
+    const int row_steps = ceil_div(p.down.k_blocks, 2), parts = split * kMoeWarps, part = rank * kMoeWarps + warp;
+    const long long steps = static_cast<long long>(lists.n_segments) * row_steps;
     long long step = steps * part / parts;
     const long long end = steps * (part + 1) / parts;
     while (step < end) {
-        const int seg = static_cast<int>(step / k_blocks), kb0 = static_cast<int>(step - static_cast<long long>(seg) * k_blocks);
-        const int kb1 = static_cast<int>(min(static_cast<long long>(k_blocks), kb0 + (end - step)));
-        step += kb1 - kb0;
+        const int seg = static_cast<int>(step / row_steps), s0 = static_cast<int>(step - static_cast<long long>(seg) * row_steps);
+        const int s1 = static_cast<int>(min(static_cast<long long>(row_steps), s0 + (end - step)));
+        step += s1 - s0;
         const Segment sg = lists.segments[seg];
-        WarpProduct<R, NT, DEPTH, G32, ZERO, SplitSource> product;
+        typename Shape::Product product;
 #pragma unroll
         for (int r = 0; r < R; ++r)
             product.set_rows(r, p.down, sg.expert, min(block0 + r, p.down.row_blocks - 1), lane);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const int pair = lists.order[sg.first + min(8 * n + lane / 4, sg.columns - 1)];
-            product.x[n] = {p.h + static_cast<size_t>(pair) * p.h_stride, p.h_low, p.h_stride};
+            const int pair = lists.order[sg.first + min(8 * n + lane / 4, sg.columns - 1)], k = 8 * (lane & 3);
+            const size_t at = static_cast<size_t>(pair) * p.h_stride + k;
+            if constexpr (sizeof(T) == 4) product.x[n] = {static_cast<const float*>(p.h) + at, p.h_stride - k, true};
+            else product.x[n] = {static_cast<const __nv_bfloat16*>(p.h) + at, p.h_stride - k, p.h_low};
         }
+        product.set_columns(p.h_stride);
         float acc[R][NT][4] = {};
-        product.run(kb0, kb1, lane, acc);
+        product.run(smem + warp * Shape::Product::kWarpBytes, s0, s1, lane, acc);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -435,79 +460,43 @@ inline int tokens_per_launch(int top_k) {
     return t < kMaxTokens ? t : kMaxTokens;
 }
 
-template <typename Kernel>
-int launch(Kernel kernel, unsigned grid, unsigned cluster, size_t smem, cudaStream_t stream, const ExpertParams& p) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid, 1, 1);
-    cfg.blockDim = dim3(kMoeThreads, 1, 1);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = cluster;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    if (cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess) return HGEMM_OK;
-    cudaGetLastError();
-    return HGEMM_ERR_CUDA;
-}
-
-template <typename T, int RH, int NT, int DEPTH, bool G32, bool ZERO>
-int launch_gate_up(const ExpertParams& p, int sms, cudaStream_t stream) {
-    auto kernel = moe_gate_up_kernel<T, RH, NT, DEPTH, G32, ZERO>;
-    static std::atomic<int> per_sm{0};  // the same on every sm_100 device
-    int b = per_sm.load(std::memory_order_relaxed);
-    if (b == 0) {
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&b, kernel, kMoeThreads, 0) != cudaSuccess || b < 1) b = 1;
-        per_sm.store(b, std::memory_order_relaxed);
-    }
+template <typename T, int RH, int NT, int STAGES, int GROUP, bool ZERO>
+int launch_gate_up(const ExpertParams& p, int sms, int dev, cudaStream_t stream) {
+    using Shape = GateUpShape<T, RH, NT, STAGES, GROUP, ZERO>;
+    constexpr auto kernel = moe_gate_up_kernel<T, RH, NT, STAGES, GROUP, ZERO>;
+    const int per_sm = resident_ctas<kernel>(dev, kMoeThreads, Shape::kSmem);
+    if (per_sm < 1) return HGEMM_ERR_CUDA;
     const int pairs = p.T * p.top_k, experts = pairs < p.E ? pairs : p.E;
     const long long most = static_cast<long long>(experts + pairs / (8 * NT)) * ceil_div(p.gate.row_blocks, RH);
-    const long long wave = static_cast<long long>(sms) * b;
-    return launch(kernel, static_cast<unsigned>(most < wave ? most : wave), 1, 0, stream, p);
+    const long long wave = static_cast<long long>(sms) * per_sm;
+    return launch<kernel>(dim3(static_cast<unsigned>(most < wave ? most : wave)), kMoeThreads, 1, Shape::kSmem, stream, p);
 }
 
-template <typename T, int R, int NT, int DEPTH, bool G32, bool ZERO>
-int launch_down(const ExpertParams& p, int sms, cudaStream_t stream) {
-    auto kernel = moe_down_kernel<T, R, NT, DEPTH, G32, ZERO>;
-    const size_t smem = DownShape<R>::smem(p.T);
-    static std::atomic<unsigned long long> ready{0};  // per device: the kernel may have its largest shared memory
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return HGEMM_ERR_NO_DEVICE;
-    if (!(ready.load(std::memory_order_relaxed) >> dev & 1)) {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 static_cast<int>(DownShape<R>::smem(kMaxTokens))) != cudaSuccess) {
-            cudaGetLastError();
-            return HGEMM_ERR_CUDA;
-        }
-        ready.fetch_or(1ull << dev, std::memory_order_relaxed);
-    }
+template <typename T, int R, int NT, int STAGES, int GROUP, bool ZERO>
+int launch_down(const ExpertParams& p, int sms, int dev, cudaStream_t stream) {
+    using Shape = DownShape<T, R, NT, STAGES, GROUP, ZERO>;
+    constexpr auto kernel = moe_down_kernel<T, R, NT, STAGES, GROUP, ZERO>;
+    if (resident_ctas<kernel>(dev, kMoeThreads, Shape::smem(kMaxTokens)) < 1) return HGEMM_ERR_CUDA;
     const int groups = ceil_div(p.down.row_blocks, R);
     int split = 1;
     while (split < 8 && groups * split < 2 * sms) split *= 2;
-    return launch(kernel, static_cast<unsigned>(groups) * split, static_cast<unsigned>(split), smem, stream, p);
+    return launch<kernel>(dim3(static_cast<unsigned>(groups) * split), kMoeThreads, split, Shape::smem(p.T), stream, p);
 }
 
-template <typename T, bool G32, bool ZERO>
-int run_gate_up(const ExpertParams& p, int sms, cudaStream_t stream) {
+template <typename T, int GROUP, bool ZERO>
+int run_gate_up(const ExpertParams& p, int sms, int dev, cudaStream_t stream) {
     if constexpr (sizeof(T) == 4) {
-        return launch_gate_up<T, 1, 1, 2, G32, ZERO>(p, sms, stream);
+        return launch_gate_up<T, 1, 1, 4, GROUP, ZERO>(p, sms, dev, stream);
     } else {
-        if (p.T * p.top_k <= 8 * p.E) return launch_gate_up<T, 1, 1, 4, G32, ZERO>(p, sms, stream);
-        return launch_gate_up<T, 1, 2, 2, G32, ZERO>(p, sms, stream);
+        if (p.T * p.top_k <= 8 * p.E) return launch_gate_up<T, 1, 1, 4, GROUP, ZERO>(p, sms, dev, stream);
+        return launch_gate_up<T, 1, 2, 4, GROUP, ZERO>(p, sms, dev, stream);
     }
 }
 
-template <typename T, bool G32, bool ZERO>
-int run_down(const ExpertParams& p, int sms, cudaStream_t stream) {
-    return launch_down<T, 2, 1, 2, G32, ZERO>(p, sms, stream);
+template <typename T, int GROUP, bool ZERO>
+int run_down(const ExpertParams& p, int sms, int dev, cudaStream_t stream) {
+    return launch_down<T, 2, 1, 3, GROUP, ZERO>(p, sms, dev, stream);
 }
-
-inline bool misaligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1u)) != 0; }
 
 inline size_t h_stride(int F) { return static_cast<size_t>(ceil_div(F, kTileRows)) * kTileRows; }
 
@@ -526,8 +515,8 @@ int hgemm_moe_route(const void* x, int x_dtype, long long ldx, const void* route
     const unsigned size = x_dtype == HGEMM_DTYPE_F32 ? 4 : 2;
     if (hgw::misaligned(x, size) || hgw::misaligned(router, size) || hgw::misaligned(ids, 4) || hgw::misaligned(weights, 4))
         return HGEMM_ERR_ALIGNMENT;
-    int sms = 0;
-    if (int rc = hgw::current_sms(&sms)) return rc;
+    int sms = 0, dev = 0;
+    if (int rc = hgw::current_device(&sms, &dev)) return rc;
     hgw::RouteParams p{x, router, T > 1 ? ldx : 0, T, D, E, top_k, renormalize != 0, false, ids, weights};
     p.vec = !hgw::misaligned(x, 16) && !hgw::misaligned(router, 16) && D % 8 == 0 && p.ldx % (16 / size) == 0;
     cudaLaunchConfig_t cfg{};
@@ -549,7 +538,7 @@ int hgemm_moe_route(const void* x, int x_dtype, long long ldx, const void* route
 size_t hgemm_w4_moe_workspace_bytes(int T, int top_k, int F) {
     if (T <= 0 || top_k <= 0 || top_k > hgw::kMaxTopK || F <= 0) return 0;
     const int most = hgw::tokens_per_launch(top_k), tokens = T < most ? T : most;
-    return static_cast<size_t>(tokens) * top_k * hgw::h_stride(F) * 4;  // two bf16 per element of h
+    return static_cast<size_t>(tokens) * top_k * hgw::h_stride(F) * 4;  // h: fp32, or two bf16
 }
 
 int hgemm_w4_moe(const void* x, int x_dtype, long long ldx, const int* ids, const float* weights, int T, int top_k, int E,
@@ -568,19 +557,19 @@ int hgemm_w4_moe(const void* x, int x_dtype, long long ldx, const int* ids, cons
     if (hgw::misaligned(x, size) || hgw::misaligned(out, size) || hgw::misaligned(ids, 4) || hgw::misaligned(weights, 4))
         return HGEMM_ERR_ALIGNMENT;
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    int sms = 0;
+    int sms = 0, dev = 0;
     if (F == 0) {
-        if (int rc = hgw::current_sms(&sms)) return rc;
+        if (int rc = hgw::current_device(&sms, &dev)) return rc;
         return cudaMemsetAsync(out, 0, static_cast<size_t>(T) * D * size, s) == cudaSuccess ? HGEMM_OK : HGEMM_ERR_CUDA;
     }
     for (const hgemm_w4_weight* w : {gate, up, down}) {
         if (!w->q || !w->scales) return HGEMM_ERR_INVALID_VALUE;
-        if (hgw::misaligned(w->q, 16) || hgw::misaligned(w->scales, 4) || hgw::misaligned(w->zeros, 2))
+        if (hgw::misaligned(w->q, 16) || hgw::misaligned(w->scales, 4) || hgw::misaligned(w->zeros, 4))
             return HGEMM_ERR_ALIGNMENT;
     }
     if (!workspace || workspace_bytes < hgemm_w4_moe_workspace_bytes(T, top_k, F)) return HGEMM_ERR_INVALID_VALUE;
     if (hgw::misaligned(workspace, 16)) return HGEMM_ERR_ALIGNMENT;
-    if (int rc = hgw::current_sms(&sms)) return rc;
+    if (int rc = hgw::current_device(&sms, &dev)) return rc;
 
     const int most = hgw::tokens_per_launch(top_k);
     hgw::ExpertParams p{};
@@ -593,15 +582,9 @@ int hgemm_w4_moe(const void* x, int x_dtype, long long ldx, const int* ids, cons
     p.up = hgw::make_weight(up->q, up->scales, up->zeros, F, D, up->group);
     p.down = hgw::make_weight(down->q, down->scales, down->zeros, D, F, down->group);
     p.vec = !hgw::misaligned(x, 16) && D % 8 == 0 && p.ldx % (16 / size) == 0;
-    p.h = static_cast<__nv_bfloat16*>(workspace);
+    p.h = workspace;
     p.h_stride = static_cast<int>(hgw::h_stride(F));
     p.h_low = static_cast<long long>(T < most ? T : most) * top_k * p.h_stride;
-    using True = std::true_type;
-    using False = std::false_type;
-    auto pick = [](const hgemm_w4_weight* w, auto go) {
-        if (w->group == 32) return w->zeros ? go(True{}, True{}) : go(True{}, False{});
-        return w->zeros ? go(False{}, True{}) : go(False{}, False{});
-    };
     // Launches of up to kMaxTokens tokens; they share the workspace, in stream order.
     for (int t0 = 0; t0 < T; t0 += most) {
         p.T = T - t0 < most ? T - t0 : most;
@@ -609,16 +592,18 @@ int hgemm_w4_moe(const void* x, int x_dtype, long long ldx, const int* ids, cons
         p.ids = ids + static_cast<size_t>(t0) * top_k;
         p.weights = weights + static_cast<size_t>(t0) * top_k;
         p.out = static_cast<char*>(out) + static_cast<size_t>(t0) * D * size;
-        int rc = pick(gate, [&](auto g, auto z) {
-            constexpr bool G = decltype(g)::value, Z = decltype(z)::value;
-            return x_dtype == HGEMM_DTYPE_F32 ? hgw::run_gate_up<float, G, Z>(p, sms, s)
-                                              : hgw::run_gate_up<__nv_bfloat16, G, Z>(p, sms, s);
+        int rc = hgw::with_format(gate->group, gate->zeros != nullptr, [&](auto g, auto z) {
+            constexpr int G = decltype(g)::value;
+            constexpr bool Z = decltype(z)::value;
+            return x_dtype == HGEMM_DTYPE_F32 ? hgw::run_gate_up<float, G, Z>(p, sms, dev, s)
+                                              : hgw::run_gate_up<__nv_bfloat16, G, Z>(p, sms, dev, s);
         });
         if (rc) return rc;
-        rc = pick(down, [&](auto g, auto z) {
-            constexpr bool G = decltype(g)::value, Z = decltype(z)::value;
-            return x_dtype == HGEMM_DTYPE_F32 ? hgw::run_down<float, G, Z>(p, sms, s)
-                                              : hgw::run_down<__nv_bfloat16, G, Z>(p, sms, s);
+        rc = hgw::with_format(down->group, down->zeros != nullptr, [&](auto g, auto z) {
+            constexpr int G = decltype(g)::value;
+            constexpr bool Z = decltype(z)::value;
+            return x_dtype == HGEMM_DTYPE_F32 ? hgw::run_down<float, G, Z>(p, sms, dev, s)
+                                              : hgw::run_down<__nv_bfloat16, G, Z>(p, sms, dev, s);
         });
         if (rc) return rc;
     }

@@ -11,27 +11,26 @@ namespace cg = cooperative_groups;
 
 namespace hgw {
 
-int current_sms(int* sms) {
-    static std::atomic<int> known[64];  // SM count + 1, or -1 for a device of another architecture
-    int dev = -1;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+int current_device(int* sms, int* dev) {
+    static std::atomic<int> known[kMaxDevices];  // SM count, or -1 for a device of another architecture
+    if (cudaGetDevice(dev) != cudaSuccess || *dev < 0 || *dev >= kMaxDevices) {
         cudaGetLastError();
         return HGEMM_ERR_NO_DEVICE;
     }
-    int v = known[dev].load(std::memory_order_relaxed);
+    int v = known[*dev].load(std::memory_order_relaxed);
     if (v == 0) {
         int major = 0, minor = 0, n = 0;
-        if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
-            cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev) != cudaSuccess ||
-            cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+        if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, *dev) != cudaSuccess ||
+            cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, *dev) != cudaSuccess ||
+            cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, *dev) != cudaSuccess) {
             cudaGetLastError();
             return HGEMM_ERR_NO_DEVICE;
         }
-        v = major == 10 && minor == 0 ? n + 1 : -1;
-        known[dev].store(v, std::memory_order_relaxed);
+        v = major == 10 && minor == 0 ? n : -1;
+        known[*dev].store(v, std::memory_order_relaxed);
     }
     if (v < 0) return HGEMM_ERR_NO_DEVICE;
-    *sms = v - 1;
+    *sms = v;
     return HGEMM_OK;
 }
 
@@ -269,35 +268,30 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_w4_kernel(const uint
 }
 
 // One wave of resident blocks at most.
-template <typename Kernel>
-int one_wave(Kernel kernel, size_t items, int sms) {
-    static std::atomic<int> per_sm{0};  // per kernel; the same on every sm_100 device
-    int b = per_sm.load(std::memory_order_relaxed);
-    if (b == 0) {
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&b, kernel, kQuantThreads, 0) != cudaSuccess || b < 1) b = 1;
-        per_sm.store(b, std::memory_order_relaxed);
-    }
+template <auto KERNEL>
+unsigned one_wave(size_t items, int sms, int dev) {
+    const int per_sm = resident_ctas<KERNEL>(dev, kQuantThreads, 0);
     const size_t blocks = (items + kQuantThreads / 32 - 1) / (kQuantThreads / 32);
-    const size_t cap = static_cast<size_t>(sms) * b;
-    return static_cast<int>(blocks < cap ? blocks : cap);
+    const size_t cap = static_cast<size_t>(sms) * (per_sm > 0 ? per_sm : 1);
+    return static_cast<unsigned>(blocks < cap ? blocks : cap);
 }
 
 template <typename T, bool ZERO>
 int run_quantize(const T* w, int count, int N, int K, int group, bool vec, uint8_t* q, uint32_t* scales, uint16_t* zeros,
-                 int sms, cudaStream_t stream) {
+                 int sms, int dev, cudaStream_t stream) {
     const int rb = ceil_div(N, kTileRows), kb = ceil_div(K, kTileK);
     const size_t items = static_cast<size_t>(count) * rb * ceil_div(kb, 2);
-    quantize_w4_kernel<T, ZERO><<<one_wave(quantize_w4_kernel<T, ZERO>, items, sms), kQuantThreads, 0, stream>>>(
+    quantize_w4_kernel<T, ZERO><<<one_wave<quantize_w4_kernel<T, ZERO>>(items, sms, dev), kQuantThreads, 0, stream>>>(
         w, N, K, rb, kb, ceil_div(K, group), group, vec, items, q, scales, zeros);
     return cudaGetLastError() == cudaSuccess ? HGEMM_OK : HGEMM_ERR_CUDA;
 }
 
 template <typename T, bool ZERO>
 int run_dequantize(const uint8_t* q, const uint32_t* scales, const uint16_t* zeros, int count, int N, int K, int group,
-                   bool vec, T* w, int sms, cudaStream_t stream) {
+                   bool vec, T* w, int sms, int dev, cudaStream_t stream) {
     const Weight v = make_weight(q, scales, zeros, N, K, group);
     const size_t items = static_cast<size_t>(count) * v.row_blocks * v.k_blocks;
-    dequantize_w4_kernel<T, ZERO><<<one_wave(dequantize_w4_kernel<T, ZERO>, items, sms), kQuantThreads, 0, stream>>>(
+    dequantize_w4_kernel<T, ZERO><<<one_wave<dequantize_w4_kernel<T, ZERO>>(items, sms, dev), kQuantThreads, 0, stream>>>(
         q, scales, zeros, N, K, v.row_blocks, v.k_blocks, v.groups, v.group_shift, vec, items, w);
     return cudaGetLastError() == cudaSuccess ? HGEMM_OK : HGEMM_ERR_CUDA;
 }
@@ -327,39 +321,51 @@ __device__ __forceinline__ void store<float>(float* p, float v) { *p = v; }
 template <>
 __device__ __forceinline__ void store<__nv_bfloat16>(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-template <typename T, int R, int NT, int DEPTH, bool G32, bool ZERO>
+// Shared memory: the warps' rings, and over them, once the products are done, their sums.
+template <typename T, int R, int NT, int STAGES, int GROUP, bool ZERO>
+struct LinearShape {
+    using Product = WarpProduct<R, NT, STAGES, GROUP, ZERO, RowSource<T>>;
+    static constexpr int kOut = R * NT * 128;  // a CTA's outputs: 16 R rows x 8 NT columns, in fragment order
+    static constexpr int kRings = kWarps * Product::kWarpBytes, kSums = kWarps * kOut * 4;
+    static constexpr int kSmem = kRings > kSums ? kRings : kSums;
+};
+
+template <typename T, int R, int NT, int STAGES, int GROUP, bool ZERO>
 __global__ void __launch_bounds__(kWarps * 32) w4_linear_kernel(const LinearParams p) {
-    constexpr int kOut = R * NT * 128;  // a CTA's outputs: 16 R rows x 8 NT columns, in fragment order
-    __shared__ float partial[kWarps][kOut];
+    using Shape = LinearShape<T, R, NT, STAGES, GROUP, ZERO>;
+    constexpr int kOut = Shape::kOut;
+    extern __shared__ __align__(16) uint8_t smem[];
+    float* partial = reinterpret_cast<float*>(smem);  // [warp][kOut]
     cg::cluster_group cluster = cg::this_cluster();
     const int split = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     const int block0 = static_cast<int>(blockIdx.x) / split * R, col0 = static_cast<int>(blockIdx.y) * 8 * NT;
 
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-
-    WarpProduct<R, NT, DEPTH, G32, ZERO, RowSource<T>> product;
+    typename Shape::Product product;
 #pragma unroll
     for (int r = 0; r < R; ++r) product.set_rows(r, p.w, 0, min(block0 + r, p.w.row_blocks - 1), lane);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         // Columns past M repeat the last row; their sums are not stored.
         const int col = min(col0 + 8 * n + lane / 4, p.M - 1);
-        product.x[n] = {static_cast<const T*>(p.x) + col * p.ldx, p.K, p.vec};
+        product.x[n] = {static_cast<const T*>(p.x) + col * p.ldx + 8 * (lane & 3), p.K - 8 * (lane & 3), p.vec};
     }
-    const int parts = split * kWarps, part = rank * kWarps + warp;
-    const int kb0 = static_cast<int>(static_cast<long long>(p.w.k_blocks) * part / parts);
-    const int kb1 = static_cast<int>(static_cast<long long>(p.w.k_blocks) * (part + 1) / parts);
+    product.set_columns(p.vec ? p.K : 0);
+    const int steps = ceil_div(p.w.k_blocks, 2), parts = split * kWarps, part = rank * kWarps + warp;
+    const int s0 = static_cast<int>(static_cast<long long>(steps) * part / parts);
+    const int s1 = static_cast<int>(static_cast<long long>(steps) * (part + 1) / parts);
     float acc[R][NT][4] = {};
-    product.run(kb0, kb1, lane, acc);
+    pdl_trigger();
+    pdl_wait();
+    product.run(smem + warp * Shape::Product::kWarpBytes, s0, s1, lane, acc);
 
+    __syncthreads();
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) partial[warp][((r * NT + n) * 4 + i) * 32 + lane] = acc[r][n][i];
+            for (int i = 0; i < 4; ++i) partial[warp * kOut + ((r * NT + n) * 4 + i) * 32 + lane] = acc[r][n][i];
     __syncthreads();
     auto finish = [&](int i, float v) {
         const int l = i & 31, f = (i >> 5) & 3, n = (i >> 7) % NT, r = (i >> 7) / NT;
@@ -367,17 +373,17 @@ __global__ void __launch_bounds__(kWarps * 32) w4_linear_kernel(const LinearPara
         if (row < p.N && col < p.M) store<T>(static_cast<T*>(p.y) + static_cast<size_t>(col) * p.N + row, v);
     };
     for (int i = threadIdx.x; i < kOut; i += kWarps * 32) {
-        float v = partial[0][i];
+        float v = partial[i];
 #pragma unroll
-        for (int w = 1; w < kWarps; ++w) v += partial[w][i];
+        for (int w = 1; w < kWarps; ++w) v += partial[w * kOut + i];
         if (split == 1) finish(i, v);
-        else partial[0][i] = v;
+        else partial[i] = v;
     }
     if (split > 1) {
         cluster.sync();
         for (int i = rank * kWarps * 32 + threadIdx.x; i < kOut; i += split * kWarps * 32) {
             float v = 0.0f;
-            for (int s = 0; s < split; ++s) v += cluster.map_shared_rank(&partial[0][0], s)[i];
+            for (int s = 0; s < split; ++s) v += cluster.map_shared_rank(partial, s)[i];
             finish(i, v);
         }
         cluster.sync();  // no CTA leaves while another reads its sums
@@ -385,54 +391,39 @@ __global__ void __launch_bounds__(kWarps * 32) w4_linear_kernel(const LinearPara
 }
 
 // CTAs of a cluster that share the K of a row group, for `groups` groups of rows: enough CTAs
-// for two on every SM, as long as a warp keeps two K blocks.
-inline int choose_split(int groups, int k_blocks, int sms) {
+// for two on every SM, as long as a warp keeps two steps.
+inline int choose_split(int groups, int steps, int sms) {
     int split = 1;
-    while (split < 8 && groups * split < 2 * sms && k_blocks >= 2 * split * kWarps * 2) split *= 2;
+    while (split < 8 && groups * split < 2 * sms && steps >= 2 * split * kWarps * 2) split *= 2;
     return split;
 }
 
-template <typename T, int R, int NT, int DEPTH, bool G32, bool ZERO>
-int launch_linear(const LinearParams& p, int sms, cudaStream_t stream) {
-    const int groups = ceil_div(p.w.row_blocks, R);
-    const int split = choose_split(groups * ceil_div(p.M, 8 * NT), p.w.k_blocks, sms);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(groups) * split, static_cast<unsigned>(ceil_div(p.M, 8 * NT)), 1);
-    cfg.blockDim = dim3(kWarps * 32, 1, 1);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(split);
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, w4_linear_kernel<T, R, NT, DEPTH, G32, ZERO>, p);
-    if (e == cudaSuccess) return HGEMM_OK;
-    cudaGetLastError();
-    return HGEMM_ERR_CUDA;
+template <typename T, int R, int NT, int STAGES, int GROUP, bool ZERO>
+int launch_linear(const LinearParams& p, int sms, int dev, cudaStream_t stream) {
+    using Shape = LinearShape<T, R, NT, STAGES, GROUP, ZERO>;
+    constexpr auto kernel = w4_linear_kernel<T, R, NT, STAGES, GROUP, ZERO>;
+    if (resident_ctas<kernel>(dev, kWarps * 32, Shape::kSmem) < 1) return HGEMM_ERR_CUDA;
+    const int groups = ceil_div(p.w.row_blocks, R), columns = ceil_div(p.M, 8 * NT);
+    const int split = choose_split(groups * columns, ceil_div(p.w.k_blocks, 2), sms);
+    return launch<kernel>(dim3(static_cast<unsigned>(groups) * split, static_cast<unsigned>(columns), 1), kWarps * 32, split,
+                          Shape::kSmem, stream, p);
 }
 
-template <typename T, bool G32, bool ZERO>
-int run_linear(const LinearParams& p, int sms, cudaStream_t stream) {
+template <typename T, int GROUP, bool ZERO>
+int run_linear(const LinearParams& p, int sms, int dev, cudaStream_t stream) {
     if constexpr (sizeof(T) == 4) {
-        return launch_linear<T, 2, 1, 2, G32, ZERO>(p, sms, stream);
+        return launch_linear<T, 2, 1, 4, GROUP, ZERO>(p, sms, dev, stream);
     } else {
-        if (p.M <= 8) return launch_linear<T, 2, 1, 4, G32, ZERO>(p, sms, stream);
-        if (p.M <= 16) return launch_linear<T, 2, 2, 2, G32, ZERO>(p, sms, stream);
-        return launch_linear<T, 2, 4, 2, G32, ZERO>(p, sms, stream);
+        if (p.M <= 8) return launch_linear<T, 2, 1, 4, GROUP, ZERO>(p, sms, dev, stream);
+        if (p.M <= 16) return launch_linear<T, 2, 2, 4, GROUP, ZERO>(p, sms, dev, stream);
+        return launch_linear<T, 2, 4, 4, GROUP, ZERO>(p, sms, dev, stream);
     }
 }
 
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-// The checks that every entry point makes of a blocked weight.
-inline int check_weight(const void* q, const void* scales, const void* zeros) {
+// The checks that every entry point makes of a blocked weight.  The products copy zero points 4 bytes at a time.
+inline int check_weight(const void* q, const void* scales, const void* zeros, unsigned zeros_align) {
     if (!q || !scales) return HGEMM_ERR_INVALID_VALUE;
-    if (!aligned16(q) || (reinterpret_cast<uintptr_t>(scales) & 3u) || (reinterpret_cast<uintptr_t>(zeros) & 1u))
-        return HGEMM_ERR_ALIGNMENT;
+    if (misaligned(q, 16) || misaligned(scales, 4) || misaligned(zeros, zeros_align)) return HGEMM_ERR_ALIGNMENT;
     return HGEMM_OK;
 }
 
@@ -456,21 +447,21 @@ int hgemm_quantize_w4(const void* w, int w_dtype, int count, int N, int K, int g
     if (w_dtype != HGEMM_DTYPE_F32 && w_dtype != HGEMM_DTYPE_BF16) return HGEMM_ERR_INVALID_VALUE;
     if (count == 0 || N == 0 || K == 0) return HGEMM_OK;
     if (!w) return HGEMM_ERR_INVALID_VALUE;
-    if (int rc = hgw::check_weight(q, scales, zeros)) return rc;
-    const int size = w_dtype == HGEMM_DTYPE_F32 ? 4 : 2;
-    if (reinterpret_cast<uintptr_t>(w) & (size - 1u)) return HGEMM_ERR_ALIGNMENT;
-    int sms = 0;
-    if (int rc = hgw::current_sms(&sms)) return rc;
-    const bool vec = hgw::aligned16(w) && K % 8 == 0;
+    if (int rc = hgw::check_weight(q, scales, zeros, 2)) return rc;
+    const unsigned size = w_dtype == HGEMM_DTYPE_F32 ? 4 : 2;
+    if (hgw::misaligned(w, size)) return HGEMM_ERR_ALIGNMENT;
+    int sms = 0, dev = 0;
+    if (int rc = hgw::current_device(&sms, &dev)) return rc;
+    const bool vec = !hgw::misaligned(w, 16) && K % 8 == 0;
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     uint8_t* const qb = static_cast<uint8_t*>(q);
     uint32_t* const sc = static_cast<uint32_t*>(scales);
     uint16_t* const z = static_cast<uint16_t*>(zeros);
     auto go = [&](auto* typed) {
         return z ? hgw::run_quantize<std::remove_const_t<std::remove_pointer_t<decltype(typed)>>, true>(
-                       typed, count, N, K, group, vec, qb, sc, z, sms, s)
+                       typed, count, N, K, group, vec, qb, sc, z, sms, dev, s)
                  : hgw::run_quantize<std::remove_const_t<std::remove_pointer_t<decltype(typed)>>, false>(
-                       typed, count, N, K, group, vec, qb, sc, z, sms, s);
+                       typed, count, N, K, group, vec, qb, sc, z, sms, dev, s);
     };
     if (w_dtype == HGEMM_DTYPE_F32) return go(static_cast<const float*>(w));
     return go(static_cast<const __nv_bfloat16*>(w));
@@ -482,20 +473,20 @@ int hgemm_dequantize_w4(const void* q, const void* scales, const void* zeros, in
     if (w_dtype != HGEMM_DTYPE_F32 && w_dtype != HGEMM_DTYPE_BF16) return HGEMM_ERR_INVALID_VALUE;
     if (count == 0 || N == 0 || K == 0) return HGEMM_OK;
     if (!w) return HGEMM_ERR_INVALID_VALUE;
-    if (int rc = hgw::check_weight(q, scales, zeros)) return rc;
-    const int size = w_dtype == HGEMM_DTYPE_F32 ? 4 : 2;
-    if (reinterpret_cast<uintptr_t>(w) & (size - 1u)) return HGEMM_ERR_ALIGNMENT;
-    int sms = 0;
-    if (int rc = hgw::current_sms(&sms)) return rc;
-    const bool vec = hgw::aligned16(w) && K % 8 == 0;
+    if (int rc = hgw::check_weight(q, scales, zeros, 2)) return rc;
+    const unsigned size = w_dtype == HGEMM_DTYPE_F32 ? 4 : 2;
+    if (hgw::misaligned(w, size)) return HGEMM_ERR_ALIGNMENT;
+    int sms = 0, dev = 0;
+    if (int rc = hgw::current_device(&sms, &dev)) return rc;
+    const bool vec = !hgw::misaligned(w, 16) && K % 8 == 0;
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const uint8_t* const qb = static_cast<const uint8_t*>(q);
     const uint32_t* const sc = static_cast<const uint32_t*>(scales);
     const uint16_t* const z = static_cast<const uint16_t*>(zeros);
     auto go = [&](auto* typed) {
         using T = std::remove_pointer_t<decltype(typed)>;
-        return z ? hgw::run_dequantize<T, true>(qb, sc, z, count, N, K, group, vec, typed, sms, s)
-                 : hgw::run_dequantize<T, false>(qb, sc, z, count, N, K, group, vec, typed, sms, s);
+        return z ? hgw::run_dequantize<T, true>(qb, sc, z, count, N, K, group, vec, typed, sms, dev, s)
+                 : hgw::run_dequantize<T, false>(qb, sc, z, count, N, K, group, vec, typed, sms, dev, s);
     };
     if (w_dtype == HGEMM_DTYPE_F32) return go(static_cast<float*>(w));
     return go(static_cast<__nv_bfloat16*>(w));
@@ -508,31 +499,28 @@ int hgemm_w4_gemm_tn(const void* x, int x_dtype, long long ldx, const void* q, c
     if (M > 1 && ldx < K) return HGEMM_ERR_INVALID_VALUE;
     if (M == 0 || N == 0) return HGEMM_OK;
     if (!y) return HGEMM_ERR_INVALID_VALUE;
-    const int size = x_dtype == HGEMM_DTYPE_F32 ? 4 : 2;
-    if (reinterpret_cast<uintptr_t>(y) & (size - 1u)) return HGEMM_ERR_ALIGNMENT;
+    const unsigned size = x_dtype == HGEMM_DTYPE_F32 ? 4 : 2;
+    if (hgw::misaligned(y, size)) return HGEMM_ERR_ALIGNMENT;
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    int sms = 0;
+    int sms = 0, dev = 0;
     if (K == 0) {
-        if (int rc = hgw::current_sms(&sms)) return rc;
+        if (int rc = hgw::current_device(&sms, &dev)) return rc;
         const size_t bytes = static_cast<size_t>(M) * N * size;
         return cudaMemsetAsync(y, 0, bytes, s) == cudaSuccess ? HGEMM_OK : HGEMM_ERR_CUDA;
     }
     if (!x) return HGEMM_ERR_INVALID_VALUE;
-    if (int rc = hgw::check_weight(q, scales, zeros)) return rc;
-    if (reinterpret_cast<uintptr_t>(x) & (size - 1u)) return HGEMM_ERR_ALIGNMENT;
-    if (int rc = hgw::current_sms(&sms)) return rc;
+    if (int rc = hgw::check_weight(q, scales, zeros, 4)) return rc;
+    if (hgw::misaligned(x, size)) return HGEMM_ERR_ALIGNMENT;
+    if (int rc = hgw::current_device(&sms, &dev)) return rc;
     if (M > 65535 * 8) return HGEMM_ERR_UNSUPPORTED;  // grid.y
     hgw::LinearParams p{x, M > 1 ? ldx : 0, y, M, N, K, hgw::make_weight(q, scales, zeros, N, K, group),
-                        hgw::aligned16(x) && K % 8 == 0 && (M == 1 || ldx % (16 / size) == 0)};
-    auto go = [&](auto g32, auto zero) {
-        constexpr bool G = decltype(g32)::value, Z = decltype(zero)::value;
-        return x_dtype == HGEMM_DTYPE_F32 ? hgw::run_linear<float, G, Z>(p, sms, s)
-                                          : hgw::run_linear<__nv_bfloat16, G, Z>(p, sms, s);
-    };
-    using True = std::true_type;
-    using False = std::false_type;
-    if (group == 32) return zeros ? go(True{}, True{}) : go(True{}, False{});
-    return zeros ? go(False{}, True{}) : go(False{}, False{});
+                        !hgw::misaligned(x, 16) && K % 8 == 0 && (M == 1 || ldx % (16 / size) == 0)};
+    return hgw::with_format(group, zeros != nullptr, [&](auto g, auto z) {
+        constexpr int G = decltype(g)::value;
+        constexpr bool Z = decltype(z)::value;
+        return x_dtype == HGEMM_DTYPE_F32 ? hgw::run_linear<float, G, Z>(p, sms, dev, s)
+                                          : hgw::run_linear<__nv_bfloat16, G, Z>(p, sms, dev, s);
+    });
 }
 
 }  // extern "C"

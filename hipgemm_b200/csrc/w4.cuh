@@ -19,14 +19,17 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
+#include <type_traits>
 
 namespace hgw {
 
 constexpr int kTileRows = 16;
 constexpr int kTileK = 64;
 constexpr int kTileBytes = 512;
+constexpr int kMaxDevices = 64;
 
 __host__ __device__ constexpr int ceil_div(int a, int b) { return a / b + (a % b != 0); }
 
@@ -66,14 +69,30 @@ __device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
     return d;
 }
 
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
 
+// The unpacking's constants, in registers that the compiler cannot see through: a logic instruction
+// takes one immediate operand, so that with both constants known it would take two of them.
+struct UnpackConstants {
+    uint32_t mask, magic;
+    __device__ __forceinline__ UnpackConstants() {
+        asm volatile("mov.b32 %0, 0x000F000F;\n\tmov.b32 %1, 0x43004300;" : "=r"(mask), "=r"(magic));
+    }
+};
+
 // Word j of a tile -> the A fragment of its 16 K: code - zero, exact.  z0 and z1 are 128 + zero
-// as two equal bf16, for rows g and g + 8.
-__device__ __forceinline__ void unpack(uint32_t w, uint32_t z0, uint32_t z1, uint32_t (&a)[4]) {
+// as two equal bf16, for rows g and g + 8.  3 shifts, 4 logic instructions, 4 subtractions.
+__device__ __forceinline__ void unpack(uint32_t w, const UnpackConstants& c, uint32_t z0, uint32_t z1, uint32_t (&a)[4]) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) a[r] = sub_bf16x2(((w >> (4 * r)) & 0x000F000Fu) | 0x43004300u, r & 1 ? z1 : z0);
+    for (int r = 0; r < 4; ++r) {
+        uint32_t v;
+        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(w >> (4 * r)), "r"(c.mask), "r"(c.magic));  // (a & b) | c
+        a[r] = sub_bf16x2(v, r & 1 ? z1 : z0);
+    }
 }
 
 // A streaming 16-byte load: each weight byte is used once per call.
@@ -87,12 +106,12 @@ __device__ __forceinline__ uint4 load_stream(const uint8_t* p) {
 
 // ---- the activations' side -----------------------------------------------------------------
 //
-// A source gives a lane its B fragments of one 64-K block: kTerms bf16 terms whose sum is x
-// (exactly, for fp32: three truncations of 8 bits each).  Raw is what is kept in registers
-// while a block is in flight.
+// A source gives a lane its B fragments of 64 K: kTerms bf16 terms whose sum is x (exactly, for
+// fp32: three truncations of 8 bits each).  Raw is what is kept in registers while it is in flight.
 
-// Rows of bf16 or fp32 in memory.  `row` points to the lane's column's row; elements at and past
-// `len` are zero (a stored pad would do for the codes, but x may hold infinities there).
+// Rows of bf16 or fp32 in memory.  `row` points to the lane's column's row, 8 (lane % 4) elements
+// in; `len` is what is left of the row there.  Elements at and past it are zero: the codes there
+// are padding that stands for anything, and what follows a row may be an infinity.
 template <typename T>
 struct RowSource;
 
@@ -104,7 +123,11 @@ struct RowSource<__nv_bfloat16> {
     };
     const __nv_bfloat16* row;
     int len;
-    bool vec;  // rows 16-byte aligned and len % 8 == 0
+    bool vec;  // rows 16-byte aligned and of a multiple of 8 elements
+    __device__ __forceinline__ void load_full(Raw& raw, int k) const {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) raw.v[h] = __ldg(reinterpret_cast<const uint4*>(row + k) + 4 * h);
+    }
     __device__ __forceinline__ void load(Raw& raw, int k) const {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -150,6 +173,13 @@ struct RowSource<float> {
     const float* row;
     int len;
     bool vec;
+    __device__ __forceinline__ void load_full(Raw& raw, int k) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 f = __ldg(reinterpret_cast<const float4*>(row + k) + (i & 1) + 8 * (i / 2));
+            raw.v[4 * i] = f.x, raw.v[4 * i + 1] = f.y, raw.v[4 * i + 2] = f.z, raw.v[4 * i + 3] = f.w;
+        }
+    }
     __device__ __forceinline__ void load(Raw& raw, int k) const {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -186,113 +216,226 @@ struct RowSource<float> {
 
 // ---- a warp's product ------------------------------------------------------------------------
 //
-// acc[r][n][.] += sum over K blocks [kb0, kb1) of rows (row block r) x columns (tile n of 8).
+// acc[r][n][.] += sum over steps [s0, s1) of 128 K of (row block r) x (columns: tile n of 8).
 // Fragment element i of lane 4 g + t is row g + 8 (i / 2), column 2 t + i % 2.
-// Per K block and row block a lane loads 16 bytes of codes and its scales; DEPTH blocks are in
-// flight.  The group's sum is scaled once per 64 K (per 32 K for groups of 32): 4 FMAs for 4
-// (2) matrix instructions.
-template <int R, int NT, int DEPTH, bool G32, bool ZERO, typename Source>
+//
+// Codes and scales come through a ring of STAGES steps in shared memory that each lane fills with
+// asynchronous copies of its own 16 (4) bytes and reads back itself: enough bytes in flight for
+// HBM without registers for them, and no barrier.  The activations, which are in L1 or L2, are
+// loaded one tile ahead.  Per tile (512 bytes of codes) a warp issues about 60 instructions, 28
+// of them logic at 2 cycles each; at HBM speed a scheduler has 86 cycles for a tile.
+
+__device__ __forceinline__ void copy16(uint32_t smem, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t smem, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+constexpr int kStepK = 128;
+
+template <int R, int NT, int STAGES, int GROUP, bool ZERO, typename Source>
 struct WarpProduct {
-    static constexpr int kScales = G32 ? 2 : 1;  // groups that start in a 64-K block
-    struct Stage {
-        uint4 q[R];
-        uint32_t scale[R][kScales];
-        uint16_t zero[R][kScales];
-        typename Source::Raw x[NT];
-    };
+    static constexpr int kGroups = kStepK / GROUP;  // groups of a step
+    static constexpr int kCodes = R * 2 * kTileBytes;
+    static constexpr int kScales = R * kGroups * 32 * 4;
+    static constexpr int kStageBytes = kCodes + kScales * (ZERO ? 2 : 1);
+    static constexpr int kWarpBytes = kStageBytes * STAGES;
 
     const uint8_t* q[R];         // this lane's 16 bytes of the row blocks' first tiles
     const uint32_t* scales[R];   // this lane's pair of the row blocks' first groups
-    const uint16_t* zeros[R];
+    const uint8_t* zeros[R];     // the 4 bytes that this lane's pair is in
     Source x[NT];
-    int group_shift, groups;
+    int k_blocks, groups;
+    int full_blocks;             // K blocks whose x is loaded without a look at the row's end
+
+    // `columns`: elements of a row of x, or 0 where its rows are not aligned.
+    __device__ __forceinline__ void set_columns(int columns) { full_blocks = columns / kTileK; }
 
     __device__ __forceinline__ void set_rows(int r, const Weight& w, int index, int row_block, int lane) {
         q[r] = w.q + w.tile_base(index, row_block) + lane * 16;
-        const size_t base = w.group_base(index, row_block) + lane / 4;
-        scales[r] = w.scales + base;
-        if (ZERO) zeros[r] = w.zeros + base;
-        group_shift = w.group_shift;
+        const size_t base = w.group_base(index, row_block);
+        scales[r] = w.scales + base + lane / 4;
+        if (ZERO) zeros[r] = reinterpret_cast<const uint8_t*>(w.zeros + base) + (lane / 8) * 4;
+        k_blocks = w.k_blocks;
         groups = w.groups;
     }
 
-    __device__ __forceinline__ void load(Stage& s, int kb, int lane) const {
+    // What is past the end of a row is not copied (a tile's second group of 32 among it): its x is 0,
+    // its scale is taken for 0 where it is used.
+    __device__ __forceinline__ void copy(uint32_t stage, int step, int lane) const {
+        const bool whole = 2 * step + 1 < k_blocks;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            s.q[r] = load_stream(q[r] + static_cast<size_t>(kb) * kTileBytes);
+            const uint8_t* from = q[r] + static_cast<size_t>(step) * (2 * kTileBytes);
+            const uint32_t to = stage + r * (2 * kTileBytes) + lane * 16;
+            copy16(to, from);
+            if (whole) copy16(to + kTileBytes, from + kTileBytes);
+            const uint32_t* scale = scales[r] + static_cast<size_t>(step) * (kGroups * 8);
+            const uint8_t* zero = ZERO ? zeros[r] + static_cast<size_t>(step) * (kGroups * 16) : nullptr;
 #pragma unroll
-            for (int i = 0; i < kScales; ++i) {
-                // The last block's second group of 32 may not exist: its codes are padding and x is 0 there.
-                int group = (kb * kTileK + 32 * i) >> group_shift;
-                if (G32 && i) group = group < groups ? group : groups - 1;
-                s.scale[r][i] = __ldg(scales[r] + static_cast<size_t>(group) * 8);
-                if (ZERO) s.zero[r][i] = __ldg(zeros[r] + static_cast<size_t>(group) * 8);
+            for (int i = 0; i < kGroups; ++i) {
+                if (i > 0 && step * kGroups + i >= groups) continue;
+                const uint32_t at = stage + kCodes + ((r * kGroups + i) * 32 + lane) * 4;
+                copy4(at, scale + 8 * i);
+                if (ZERO) copy4(at + kScales, zero + 16 * i);
             }
         }
+    }
+    __device__ __forceinline__ void load_x(typename Source::Raw (&raw)[NT], int block) const {
+        if (block < full_blocks) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) x[n].load(s.x[n], kb * kTileK + 8 * (lane & 3));
+            for (int n = 0; n < NT; ++n) x[n].load_full(raw[n], block * kTileK);
+        } else {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) x[n].load(raw[n], block * kTileK);
+        }
     }
 
-    __device__ __forceinline__ static void compute(const Stage& s, float (&acc)[R][NT][4]) {
+    // One tile of 64 K (half h of a step) of all row blocks.
+    template <int H>
+    __device__ __forceinline__ void tile(const UnpackConstants& c, const uint8_t* stage, int step, int lane, const typename Source::Raw (&raw)[NT],
+                                         float (&sum)[R][NT][4], float (&acc)[R][NT][4]) const {
         uint32_t b[NT][Source::kTerms][8];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) Source::terms(s.x[n], b[n]);
+        for (int n = 0; n < NT; ++n) Source::terms(raw[n], b[n]);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const uint32_t words[4] = {s.q[r].x, s.q[r].y, s.q[r].z, s.q[r].w};
-            float sum[NT][4];
+            const uint4 codes = *reinterpret_cast<const uint4*>(stage + (2 * r + H) * kTileBytes + lane * 16);
+            const uint32_t words[4] = {codes.x, codes.y, codes.z, codes.w};
+            uint32_t z0 = 0x43084308u, z1 = 0x43084308u;  // 128 + 8
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int i = G32 ? j / 2 : 0;
-                uint32_t z0 = 0x43084308u, z1 = 0x43084308u;  // 128 + 8
-                if (ZERO) {
-                    z0 = 0x43004300u | (s.zero[r][i] & 0xFFu) * 0x10001u;
-                    z1 = 0x43004300u | (s.zero[r][i] >> 8) * 0x10001u;
+                const int i = (64 * H + 16 * j) / GROUP;  // the group, of the step's
+                const uint8_t* at = stage + kCodes + ((r * kGroups + i) * 32 + lane) * 4;
+                const bool first = (64 * H + 16 * j) % GROUP == 0, last = (64 * H + 16 * j + 16) % GROUP == 0;
+                if (ZERO && (j == 0 || first)) {
+                    const uint32_t pair = *reinterpret_cast<const uint32_t*>(at + kScales) >> (lane & 4 ? 16 : 0);
+                    z0 = __byte_perm(pair, 0x43u, 0x4040);
+                    z1 = __byte_perm(pair, 0x43u, 0x4141);
                 }
                 uint32_t a[4];
-                unpack(words[j], z0, z1, a);
+                unpack(words[j], c, z0, z1, a);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    if (j == 0 || (G32 && j == 2)) sum[n][0] = sum[n][1] = sum[n][2] = sum[n][3] = 0.0f;
+                    if (first) sum[r][n][0] = sum[r][n][1] = sum[r][n][2] = sum[r][n][3] = 0.0f;
 #pragma unroll
-                    for (int t = Source::kTerms - 1; t >= 0; --t)
-                        mma_bf16(sum[n], a, b[n][t][2 * j], b[n][t][2 * j + 1]);
+                    for (int t = Source::kTerms - 1; t >= 0; --t) mma_bf16(sum[r][n], a, b[n][t][2 * j], b[n][t][2 * j + 1]);
                 }
-                if (j == 3 || (G32 && j == 1)) {
-                    const float s0 = bf16_lo(s.scale[r][i]), s1 = bf16_hi(s.scale[r][i]);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        acc[r][n][0] = fmaf(s0, sum[n][0], acc[r][n][0]);
-                        acc[r][n][1] = fmaf(s0, sum[n][1], acc[r][n][1]);
-                        acc[r][n][2] = fmaf(s1, sum[n][2], acc[r][n][2]);
-                        acc[r][n][3] = fmaf(s1, sum[n][3], acc[r][n][3]);
-                    }
-                }
+                if (last) flush(i, step, *reinterpret_cast<const uint32_t*>(at), sum[r], acc[r]);
             }
         }
     }
-
-    __device__ __forceinline__ void run(int kb0, int kb1, int lane, float (&acc)[R][NT][4]) const {
-        Stage s[DEPTH];
+    __device__ __forceinline__ void flush(int i, int step, uint32_t pair, const float (&sum)[NT][4], float (&acc)[NT][4]) const {
+        if (GROUP == 32 && i > 0) pair = step * kGroups + i < groups ? pair : 0u;
+        const float s0 = bf16_lo(pair), s1 = bf16_hi(pair);
 #pragma unroll
-        for (int d = 0; d < DEPTH; ++d)
-            if (kb0 + d < kb1) load(s[d], kb0 + d, lane);
-        for (int kb = kb0; kb < kb1; kb += DEPTH) {
-#pragma unroll
-            for (int d = 0; d < DEPTH; ++d) {
-                if (kb + d < kb1) {
-                    compute(s[d], acc);
-                    if (kb + d + DEPTH < kb1) load(s[d], kb + d + DEPTH, lane);
-                }
-            }
+        for (int n = 0; n < NT; ++n) {
+            acc[n][0] = fmaf(s0, sum[n][0], acc[n][0]);
+            acc[n][1] = fmaf(s0, sum[n][1], acc[n][1]);
+            acc[n][2] = fmaf(s1, sum[n][2], acc[n][2]);
+            acc[n][3] = fmaf(s1, sum[n][3], acc[n][3]);
         }
+    }
+
+    // `ring`: this warp's kWarpBytes of shared memory, 16-byte aligned.
+    __device__ __forceinline__ void run(uint8_t* ring, int s0, int s1, int lane, float (&acc)[R][NT][4]) const {
+        const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+#pragma unroll
+        for (int d = 0; d < STAGES - 1; ++d) {
+            if (s0 + d < s1) copy(base + d * kStageBytes, s0 + d, lane);
+            copy_commit();
+        }
+        typename Source::Raw raw[2][NT];
+        if (s0 < s1) load_x(raw[0], 2 * s0);
+        const UnpackConstants c;
+        int at = 0;  // the stage's place in the ring
+        for (int step = s0; step < s1; ++step) {
+            const int ahead = step + STAGES - 1;
+            const int into = at == 0 ? STAGES - 1 : at - 1;
+            if (ahead < s1) copy(base + into * kStageBytes, ahead, lane);
+            copy_commit();
+            copy_wait<STAGES - 1>();
+            const uint8_t* stage = ring + at * kStageBytes;
+            float sum[R][NT][4];
+            load_x(raw[1], 2 * step + 1);
+            tile<0>(c, stage, step, lane, raw[0], sum, acc);
+            const bool more = 2 * step + 1 < k_blocks;
+            if (step + 1 < s1) load_x(raw[0], 2 * step + 2);
+            if (more) {
+                tile<1>(c, stage, step, lane, raw[1], sum, acc);
+            } else if (GROUP == 128) {
+                // The row ends with half a group.
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                    flush(0, step, *reinterpret_cast<const uint32_t*>(stage + kCodes + (r * 32 + lane) * 4), sum[r], acc[r]);
+            }
+            at = at == STAGES - 1 ? 0 : at + 1;
+        }
+        copy_wait<0>();
     }
 };
 
 // ---- host side ---------------------------------------------------------------------------
 
-// SM count of the current device; a negative HGEMM_ERR_* code when there is none or it is not
-// an sm_100.  Defined in w4.cu.
-int current_sms(int* sms);
+// SM count of the current device and its number; a negative HGEMM_ERR_* code when there is none
+// or it is not an sm_100.  Defined in w4.cu.
+int current_device(int* sms, int* dev);
+
+// Lets KERNEL have `bytes` of dynamic shared memory on device `dev` (once per device), and gives the
+// CTAs of `threads` that an SM keeps resident.  0 on failure.
+template <auto KERNEL>
+int resident_ctas(int dev, int threads, size_t bytes) {
+    static std::atomic<int> known[kMaxDevices];
+    int n = known[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+        if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) != cudaSuccess ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, threads, bytes) != cudaSuccess) {
+            cudaGetLastError();
+            return 0;
+        }
+        known[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
+// Launches KERNEL with a cluster of `cluster` CTAs.  Programmatic dependent launch: the CTAs may start while the
+// stream's previous kernel ends; they touch global memory only after griddepcontrol.wait.
+template <auto KERNEL, typename Params>
+int launch(dim3 grid, int threads, int cluster, size_t smem, cudaStream_t stream, const Params& p) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    if (cudaLaunchKernelEx(&cfg, KERNEL, p) == cudaSuccess) return 0;
+    cudaGetLastError();
+    return -4;  // HGEMM_ERR_CUDA
+}
+
+inline bool misaligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1u)) != 0; }
+
+// Calls go(std::integral_constant<int, GROUP>, std::bool_constant<ZERO>) for a weight's group size and kind.
+template <typename Go>
+int with_format(int group, bool zeros, Go go) {
+    using std::integral_constant;
+    if (group == 32) return zeros ? go(integral_constant<int, 32>{}, std::true_type{}) : go(integral_constant<int, 32>{}, std::false_type{});
+    if (group == 64) return zeros ? go(integral_constant<int, 64>{}, std::true_type{}) : go(integral_constant<int, 64>{}, std::false_type{});
+    return zeros ? go(integral_constant<int, 128>{}, std::true_type{}) : go(integral_constant<int, 128>{}, std::false_type{});
+}
 
 }  // namespace hgw
