@@ -564,7 +564,7 @@ int hgemm_w4_moe(const void* x, int x_dtype, long long ldx, const int* ids, cons
     }
     for (const hgemm_w4_weight* w : {gate, up, down}) {
         if (!w->q || !w->scales) return HGEMM_ERR_INVALID_VALUE;
-        if (hgw::misaligned(w->q, 16) || hgw::misaligned(w->scales, 4) || hgw::misaligned(w->zeros, 4))
+        if (hgw::misaligned(w->q, 16) || hgw::misaligned(w->scales, 16) || hgw::misaligned(w->zeros, 16))
             return HGEMM_ERR_ALIGNMENT;
     }
     if (!workspace || workspace_bytes < hgemm_w4_moe_workspace_bytes(T, top_k, F)) return HGEMM_ERR_INVALID_VALUE;

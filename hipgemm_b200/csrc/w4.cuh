@@ -381,6 +381,336 @@ struct WarpProduct {
     }
 };
 
+// ---- a warp's product with the activations held as whole numbers ---------------------------------
+//
+// For up to 16 rows of x the products above are bound by instructions: 28 logic instructions and 16
+// subtractions per 512 bytes of codes to make bf16 of them.  As bytes the codes need 12: (w ^ 0x88..)
+// & 0xF0.. is 16 (code - 8) of the four high nibbles as signed bytes, and the same of w << 4 that of
+// the low ones; with integer tensor instructions the sums are exact as well.  So x is turned into
+// whole numbers, once: a warp keeps its K slice of x (XS steps of 128) in registers for all the row
+// blocks it goes through.  With 2^e the slice's scale, |x| < 2^e for all of a row's slice,
+//     x = 2^(e - 7) (i0 + 2^-7 i1 + 2^-14 i2 [+ 2^-21 i3]),   |i| <= 128
+// to half of the last place: 2^-21 of the slice's largest element from three planes (bf16), 2^-28
+// from four (fp32).  bf16 elements down to 2^-13 of the largest, and fp32 ones down to 2^-4, are
+// exact; what is lost of smaller ones is less than fp32 sums over the slice lose.  A slice with an
+// infinity, a NaN or an extreme exponent is computed from x itself (direct()).
+//
+// Columns: up to two rows of x take one tile, column 4 m + plane; else plane p of rows 8 m ..
+// 8 m + 7 is tile P m + p, and the planes are put together in the same lane.
+
+__device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const int (&c)[4]) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, "
+        "%13};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
+}
+
+// 1.5 * 2^23: its bits plus a whole number n, |n| < 2^22, are the bits of 1.5 * 2^23 + n.
+constexpr int kMagicBits = 0x4B400000;
+constexpr float kMagic = 12582912.0f;
+
+template <typename T>
+__device__ __forceinline__ float raw_element(const typename RowSource<T>::Raw& raw, int i);
+template <>
+__device__ __forceinline__ float raw_element<float>(const RowSource<float>::Raw& raw, int i) {
+    return raw.v[i];
+}
+template <>
+__device__ __forceinline__ float raw_element<__nv_bfloat16>(const RowSource<__nv_bfloat16>::Raw& raw, int i) {
+    const uint4 v = raw.v[i / 8];
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    return i & 1 ? bf16_hi(w[i % 8 / 2]) : bf16_lo(w[i % 8 / 2]);
+}
+
+// MT = 0: up to two rows of x in one tile; else 8 MT rows.
+template <typename T, int MT, int XS, int STAGES, int GROUP, bool ZERO>
+struct WarpStationary {
+    static constexpr bool kPacked = MT == 0;
+    static constexpr int kRowTiles = kPacked ? 1 : MT;
+    static constexpr int kPlanes = sizeof(T) == 4 ? 4 : 3;
+    static constexpr int kTiles = kPacked ? 1 : MT * kPlanes;  // tiles of plane columns
+    static constexpr int kColumns = kPacked ? 2 : 8 * MT;
+    static constexpr int kGroups = kStepK / GROUP;
+    static constexpr int kCodes = XS * 2 * kTileBytes;
+    static constexpr int kScales = XS * kGroups * 32;  // a group: 8 pairs of bf16, then (ZERO) 8 pairs of bytes
+    static constexpr int kStageBytes = kCodes + (ZERO ? kScales * 3 / 2 : kScales);
+    static constexpr int kSumBytes = ZERO ? XS * kGroups * kTiles * 8 * 4 : 0;  // sums of x by group and column
+    static constexpr int kWarpBytes = kStageBytes * STAGES + kSumBytes;
+    static constexpr int kSumStride = 20;  // floats from column to column of a warp's result: no bank conflicts
+    static constexpr int kResult = kColumns * kSumStride;
+
+    struct Rows {
+        RowSource<T> tile[kRowTiles];  // rows of x by B fragment column
+    };
+    Rows x;
+    uint32_t b[XS][4][kTiles][2];
+    float factor[kRowTiles][2];      // 2^(e - 11) of columns 2 t, 2 t + 1 (of a plane's, if packed)
+    bool special;
+    int block0, blocks;              // K blocks of the slice
+    uint8_t* ring;
+    float* x_sums;
+
+    // K blocks [first, first + 2 XS); those past `k_blocks` do not exist.
+    __device__ __forceinline__ void set_slice(uint8_t* warp_smem, int first, int k_blocks, int lane) {
+        ring = warp_smem;
+        x_sums = reinterpret_cast<float*>(warp_smem + kStageBytes * STAGES);
+        block0 = first;
+        blocks = min(2 * XS, max(0, k_blocks - first));
+        // Scales that are never copied stand for groups past the end of a row.
+        for (int s = 0; s < STAGES; ++s)
+            for (int i = lane * 4; i < kStageBytes - kCodes; i += 128)
+                *reinterpret_cast<uint32_t*>(ring + s * kStageBytes + kCodes + i) = 0u;
+        __syncwarp();
+    }
+
+    // Turns the slice of x into planes.  `full_blocks`: K blocks loaded without a look at the row's end.
+    __device__ __forceinline__ void convert(int full_blocks, int lane) {
+        special = false;
+        auto load = [&](typename RowSource<T>::Raw& raw, int m, int i) {
+            if (block0 + i < full_blocks) x.tile[m].load_full(raw, (block0 + i) * kTileK);
+            else x.tile[m].load(raw, (block0 + i) * kTileK);
+        };
+        typename RowSource<T>::Raw raw;
+#pragma unroll
+        for (int m = 0; m < kRowTiles; ++m) {
+            // Once for the largest element, once more (from L1) for the planes: the slice does not fit the registers.
+            float top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 2 * XS; ++i) {
+                load(raw, m, i);
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(raw_element<T>(raw, j))));
+            }
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) {
+                const float other = __shfl_xor_sync(0xffffffffu, top, o);
+                asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(other));
+            }
+            // top < 2^e, e = exponent - 126: x * 2^(7 - e) is below 128.
+            int exponent = static_cast<int>(__float_as_uint(top) >> 23);
+            special |= top != 0.0f && (exponent < 40 || exponent > 230);
+            exponent = min(max(exponent, 40), 230);
+            const float up = __uint_as_float(static_cast<uint32_t>(260 - exponent) << 23);     // 2^(133 - exponent)
+            float down = __uint_as_float(static_cast<uint32_t>(exponent - 10) << 23);          // 2^(exponent - 137): and 16 less
+            if (kPacked) {
+                // Lane 4 g + t has plane g % 4 of row g / 4; the factor is that of the plane.
+                const int plane = lane / 4 % 4;
+                down *= __uint_as_float(static_cast<uint32_t>(127 - 7 * plane) << 23);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) factor[m][i] = __shfl_sync(0xffffffffu, down, 4 * (2 * (lane & 3) + i));
+#pragma unroll
+            for (int i = 0; i < 2 * XS; ++i) {
+                load(raw, m, i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {  // 4 elements: one register of each plane
+                    float r[4];
+#pragma unroll
+                    for (int l = 0; l < 4; ++l) r[l] = raw_element<T>(raw, 4 * j + l) * up;
+                    uint32_t mine = 0u;
+#pragma unroll
+                    for (int p = 0; p < kPlanes; ++p) {
+                        uint32_t n[4];
+#pragma unroll
+                        for (int l = 0; l < 4; ++l) {
+                            // 128 does not fit: 127, and the next plane has the rest.
+                            const float whole = fminf(r[l] + kMagic, kMagic + 127.0f);
+                            n[l] = __float_as_uint(whole);
+                            r[l] = (r[l] - (whole - kMagic)) * 128.0f;
+                        }
+                        // The codes' order in a word: k, k + 2, k + 1, k + 3.
+                        const uint32_t word = __byte_perm(__byte_perm(n[0], n[2], 0x0040), __byte_perm(n[1], n[3], 0x0040), 0x5410);
+                        if (kPacked) mine = p == lane / 4 % 4 ? word : mine;
+                        else b[i / 2][i % 2 * 2 + j / 2][m * kPlanes + p][j % 2] = word;
+                    }
+                    if (kPacked) b[i / 2][i % 2 * 2 + j / 2][0][j % 2] = mine;
+                }
+            }
+        }
+        special = __any_sync(0xffffffffu, special);
+        if (ZERO) {
+            const uint32_t ones[4] = {0x10101010u, 0x10101010u, 0x10101010u, 0x10101010u};
+#pragma unroll
+            for (int g = 0; g < XS * kGroups; ++g)
+#pragma unroll
+                for (int n = 0; n < kTiles; ++n) {
+                    int sum[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int c = 0; c < GROUP / 32; ++c) {
+                        const int at = g * (GROUP / 32) + c;
+                        mma_s8(sum, ones, b[at / 4][at % 4][n][0], b[at / 4][at % 4][n][1], sum);
+                    }
+                    if (lane < 4)
+                        *reinterpret_cast<float2*>(x_sums + (g * kTiles + n) * 8 + 2 * lane) =
+                            make_float2(static_cast<float>(sum[0]), static_cast<float>(sum[1]));
+                }
+            __syncwarp();
+        }
+    }
+
+    // Starts the copies of the slice of one row block.  q: this lane's 16 bytes of the row block's first tile; scales,
+    // zeros: the row block's first group.  A lane copies 16 bytes of the scales, and of the zero points, for all.
+    __device__ __forceinline__ void copy(int stage, const uint8_t* q, const uint8_t* scales, const uint8_t* zeros, int groups,
+                                         int lane) const {
+        static_assert(XS * kGroups <= 16, "one copy a lane");
+        const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + stage * kStageBytes;
+        q += static_cast<size_t>(block0) * kTileBytes;
+#pragma unroll
+        for (int i = 0; i < 2 * XS; ++i)
+            if (i < blocks) copy16(base + i * kTileBytes + lane * 16, q + i * kTileBytes);
+        const int group0 = block0 / 2 * kGroups;
+        if (lane < XS * kGroups * 2 && group0 + lane / 2 < groups)
+            copy16(base + kCodes + lane * 16, scales + static_cast<size_t>(group0) * 32 + lane * 16);
+        if (ZERO && lane < XS * kGroups && group0 + lane < groups)
+            copy16(base + kCodes + kScales + lane * 16, zeros + static_cast<size_t>(group0) * 16 + lane * 16);
+    }
+
+    // The row block in `stage`: 16 rows x kColumns sums, written to result[column * kSumStride + row].
+    __device__ __forceinline__ void compute(int stage, uint32_t flip, uint32_t high, float* result, int lane) const {
+        const uint8_t* in = ring + stage * kStageBytes;
+        if (special) {
+            direct(in, x, block0, blocks, result, lane);
+            return;
+        }
+        float acc[kRowTiles][4];
+#pragma unroll
+        for (int m = 0; m < kRowTiles; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.0f;
+        const int magic[4] = {kMagicBits, kMagicBits, kMagicBits, kMagicBits};
+        int sum[kTiles][4];
+#pragma unroll
+        for (int i = 0; i < 2 * XS; ++i) {
+            const uint4 codes = *reinterpret_cast<const uint4*>(in + i * kTileBytes + lane * 16);
+            const uint32_t words[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t a[4];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t w = words[2 * h + j];
+                    asm("lop3.b32 %0, %1, %2, %3, 0x28;" : "=r"(a[2 * j]) : "r"(w << 4), "r"(flip), "r"(high));  // (a ^ b) & c
+                    asm("lop3.b32 %0, %1, %2, %3, 0x28;" : "=r"(a[2 * j + 1]) : "r"(w), "r"(flip), "r"(high));
+                }
+                const int k32 = 2 * i + h;  // of the slice
+                const bool first = k32 * 32 % GROUP == 0, last = (k32 + 1) * 32 % GROUP == 0;
+#pragma unroll
+                for (int n = 0; n < kTiles; ++n)
+                    {
+                    if (first) mma_s8(sum[n], a, b[i / 2][k32 % 4][n][0], b[i / 2][k32 % 4][n][1], magic);
+                    else mma_s8(sum[n], a, b[i / 2][k32 % 4][n][0], b[i / 2][k32 % 4][n][1], sum[n]);
+                }
+                if (last) flush(in, k32 * 32 / GROUP, sum, acc, lane);
+            }
+        }
+        if (kPacked) {
+            // Columns 4 m + plane: lanes 2 m and 2 m + 1 of four have two planes each.
+            float v0 = acc[0][0] + acc[0][1], v1 = acc[0][2] + acc[0][3];
+            v0 += __shfl_xor_sync(0xffffffffu, v0, 1);
+            v1 += __shfl_xor_sync(0xffffffffu, v1, 1);
+            if ((lane & 1) == 0) {
+                float* at = result + (lane & 3) / 2 * kSumStride + lane / 4;
+                at[0] = v0;
+                at[8] = v1;
+            }
+        } else {
+            write(result, acc, lane);
+        }
+    }
+
+private:
+    // acc += scale * 2^(e - 7) * sum over the group of (code - zero) * (the planes).
+    __device__ __forceinline__ void flush(const uint8_t* in, int group, const int (&sum)[kTiles][4], float (&acc)[kRowTiles][4],
+                                          int lane) const {
+        const uint32_t pair = *reinterpret_cast<const uint32_t*>(in + kCodes + group * 32 + lane / 4 * 4);
+        const float scale[2] = {bf16_lo(pair), bf16_hi(pair)};
+        float shift[2] = {0.0f, 0.0f};  // 8 - zero
+        if (ZERO) {
+            const uint32_t z = *reinterpret_cast<const uint16_t*>(in + kCodes + kScales + group * 16 + lane / 4 * 2);
+            // 2^23 + 0..255 as bits.
+            shift[0] = (8388608.0f + 8.0f) - __uint_as_float(__byte_perm(z, 0x4B000000u, 0x7550));
+            shift[1] = (8388608.0f + 8.0f) - __uint_as_float(__byte_perm(z, 0x4B000000u, 0x7551));
+        }
+#pragma unroll
+        for (int m = 0; m < kRowTiles; ++m) {
+            float v[4];
+#pragma unroll
+            for (int p = kPacked ? 0 : kPlanes - 1; p >= 0; --p) {
+                const int n = kPacked ? 0 : m * kPlanes + p;
+                float2 sums;
+                if (ZERO) sums = *reinterpret_cast<const float2*>(x_sums + (group * kTiles + n) * 8 + 2 * (lane & 3));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float u = __int_as_float(sum[n][i]) - kMagic;
+                    if (ZERO) u = fmaf(shift[i / 2], i % 2 ? sums.y : sums.x, u);
+                    v[i] = kPacked || p == kPlanes - 1 ? u : fmaf(v[i], 0x1p-7f, u);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[m][i] = fmaf(scale[i / 2], v[i] * factor[m][i % 2], acc[m][i]);
+        }
+    }
+
+    __device__ __forceinline__ static void write(float* result, const float (&acc)[kRowTiles][4], int lane) {
+#pragma unroll
+        for (int m = 0; m < kRowTiles; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                int column = 8 * m + 2 * (lane & 3) + i % 2;
+                if (kPacked) {  // row of x: column / 4
+                    if (column % 4 != 0) continue;
+                    column /= 4;
+                }
+                result[column * kSumStride + lane / 4 + 8 * (i / 2)] = acc[m][i];
+            }
+    }
+
+    // The same from x as it is: bf16 (or three bf16 of fp32) products as WarpProduct's.  Not inlined, and not a
+    // member that would want the planes in memory.
+    __device__ __noinline__ static void direct(const uint8_t* in, Rows x, int block0, int blocks, float* result, int lane) {
+        constexpr int kTerms = RowSource<T>::kTerms;
+        const UnpackConstants c;
+        float acc[kRowTiles][4] = {};
+        for (int i = 0; i < blocks; ++i) {
+            uint32_t terms[kRowTiles][kTerms][8];
+#pragma unroll
+            for (int m = 0; m < kRowTiles; ++m) {
+                typename RowSource<T>::Raw raw;
+                x.tile[m].load(raw, (block0 + i) * kTileK);
+                RowSource<T>::terms(raw, terms[m]);
+            }
+            const uint4 codes = *reinterpret_cast<const uint4*>(in + i * kTileBytes + lane * 16);
+            const uint32_t words[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int group = (i * kTileK + 32 * h) / GROUP;
+                const uint32_t pair = *reinterpret_cast<const uint32_t*>(in + kCodes + group * 32 + lane / 4 * 4);
+                uint32_t z0 = 0x43084308u, z1 = 0x43084308u;
+                if (ZERO) {
+                    const uint32_t z = *reinterpret_cast<const uint16_t*>(in + kCodes + kScales + group * 16 + lane / 4 * 2);
+                    z0 = __byte_perm(z, 0x43u, 0x4040);
+                    z1 = __byte_perm(z, 0x43u, 0x4141);
+                }
+                float sum[kRowTiles][4] = {};
+#pragma unroll
+                for (int j = 2 * h; j < 2 * h + 2; ++j) {
+                    uint32_t a[4];
+                    unpack(words[j], c, z0, z1, a);
+#pragma unroll
+                    for (int m = 0; m < kRowTiles; ++m)
+#pragma unroll
+                        for (int t = kTerms - 1; t >= 0; --t) mma_bf16(sum[m], a, terms[m][t][2 * j], terms[m][t][2 * j + 1]);
+                }
+#pragma unroll
+                for (int m = 0; m < kRowTiles; ++m)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) acc[m][k] = fmaf(k < 2 ? bf16_lo(pair) : bf16_hi(pair), sum[m][k], acc[m][k]);
+            }
+        }
+        write(result, acc, lane);
+    }
+};
+
 // ---- host side ---------------------------------------------------------------------------
 
 // SM count of the current device and its number; a negative HGEMM_ERR_* code when there is none

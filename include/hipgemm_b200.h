@@ -280,9 +280,9 @@ int hgemm_quantize_mx_e4m3(const void* x, int x_dtype, int rows, int K, void* q,
  *           [row block][K block]; byte 16 (4 g + t) + 4 (2 jg + jk) + 2 half + rk of a block holds
  *           the codes of k = 32 jg + 8 t + 4 jk + 2 rk + half in row g (low nibble) and row g + 8
  *           (high nibble), g = 0..7, t = 0..3, the others 0..1.  Padding may hold anything.
- *   scales  hgemm_w4_scales(N, K, group) bf16, 4-byte aligned: [row block][group][g][2], rows g
- *           and g + 8 of the block.
- *   zeros   as many bytes in the same order, 2-byte aligned, or NULL.
+ *   scales  hgemm_w4_scales(N, K, group) bf16: [row block][group][g][2], rows g and g + 8 of the
+ *           block; 16-byte aligned for the products, 4-byte for the quantiser and its inverse.
+ *   zeros   as many bytes in the same order, 16-byte (2-byte) aligned, or NULL.
  * A stack of `count` matrices (experts) is their buffers back to back. */
 size_t hgemm_w4_q_bytes(int N, int K);
 size_t hgemm_w4_scales(int N, int K, int group);
