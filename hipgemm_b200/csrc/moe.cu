@@ -27,13 +27,12 @@ constexpr int kMaxSegments = kMaxPairs;
 
 // ---- router -----------------------------------------------------------------------------
 //
-// A cluster of 8 CTAs takes kRouteTokens tokens; its 64 warps split the experts, each warp a dot
-// product over D for all of the cluster's tokens.  Eight fp32 products a lane are summed in fp32
-// and then added in 64 bits, so that experts whose logits are close are ordered as the exact
-// logits are.  The logits go to the CTA that selects the token's experts over distributed shared
-// memory.
+// A cluster of 8 CTAs takes TT tokens; its 64 warps split the experts, EW at a time, so that a
+// load of x serves EW experts and one of the router TT tokens.  Sixteen products a lane are summed
+// in fp32 and then added in 64 bits, so that experts whose logits are close are ordered as the
+// exact logits are.  The logits go to the CTA that selects the token's experts over distributed
+// shared memory.
 
-constexpr int kRouteTokens = 4;
 constexpr int kRouteCluster = 8;
 
 struct RouteParams {
@@ -46,10 +45,14 @@ struct RouteParams {
     float* weights;
 };
 
+// 8 elements of a row; zeros at and past `len`.
 template <typename T>
 __device__ __forceinline__ void route_load8(const T* row, int at, int len, bool vec, float (&v)[8]) {
     if (vec) {
-        if constexpr (sizeof(T) == 4) {
+        if (at >= len) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        } else if constexpr (sizeof(T) == 4) {
             const float4 a = __ldg(reinterpret_cast<const float4*>(row + at));
             const float4 b = __ldg(reinterpret_cast<const float4*>(row + at) + 1);
             v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
@@ -75,85 +78,142 @@ __device__ __forceinline__ unsigned long long order_key(double v) {
     return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
 
-template <typename T>
+// Sums v[i] over the lanes: afterwards v[0] of lane l is the sum of v[l / (32 / N)].
+template <int N>
+__device__ __forceinline__ void reduce_lanes(double (&v)[N], int lane) {
+#pragma unroll
+    for (int o = 16, n = N; o > 0; o >>= 1) {
+        if (n > 1) {
+            const bool upper = (lane & o) != 0;
+            n /= 2;
+#pragma unroll
+            for (int i = 0; i < n; ++i) {
+                const double keep = upper ? v[n + i] : v[i], give = upper ? v[i] : v[n + i];
+                v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+            }
+        } else {
+            v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+        }
+    }
+}
+
+template <typename T, int EW, int TT>
 __global__ void __launch_bounds__(kMoeThreads) __cluster_dims__(kRouteCluster, 1, 1) moe_route_kernel(const RouteParams p) {
     __shared__ double logits[kMaxExperts];  // of the token that this CTA selects for
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = static_cast<int>(cluster.block_rank());
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-    const int t0 = static_cast<int>(blockIdx.x) / kRouteCluster * kRouteTokens;
+    const int t0 = static_cast<int>(blockIdx.x) / kRouteCluster * TT;
     pdl_trigger();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     pdl_wait();
-    cluster.sync();  // every CTA of the cluster runs before its shared memory is written
 
-    const T* x[kRouteTokens];
+    const T* x[TT];
 #pragma unroll
-    for (int t = 0; t < kRouteTokens; ++t) x[t] = static_cast<const T*>(p.x) + min(t0 + t, p.T - 1) * p.ldx;
-    for (int e = rank * kMoeWarps + warp; e < p.E; e += kRouteCluster * kMoeWarps) {
-        const T* r = static_cast<const T*>(p.router) + static_cast<size_t>(e) * p.D;
-        double sum[kRouteTokens] = {};
-        for (int d = lane * 8; d < p.D; d += 256) {
-            float w[8];
-            route_load8<T>(r, d, p.D, p.vec, w);
+    for (int t = 0; t < TT; ++t) x[t] = static_cast<const T*>(p.x) + min(t0 + t, p.T - 1) * p.ldx;
+    bool started = false;
+    for (int e0 = (rank * kMoeWarps + warp) * EW; e0 < p.E; e0 += kRouteCluster * kMoeWarps * EW) {
+        const T* r[EW];
 #pragma unroll
-            for (int t = 0; t < kRouteTokens; ++t) {
-                float v[8], s = 0.0f;
-                route_load8<T>(x[t], d, p.D, p.vec, v);
+        for (int e = 0; e < EW; ++e) r[e] = static_cast<const T*>(p.router) + static_cast<size_t>(min(e0 + e, p.E - 1)) * p.D;
+        double sum[EW * TT] = {};
+        for (int d = lane * 8; d < p.D; d += 512) {
+            float part[EW * TT] = {};
 #pragma unroll
-                for (int i = 0; i < 8; ++i) s = fmaf(w[i], v[i], s);
-                sum[t] += static_cast<double>(s);
+            for (int half = 0; half < 2; ++half) {
+                float w[EW][8], v[TT][8];
+#pragma unroll
+                for (int e = 0; e < EW; ++e) route_load8<T>(r[e], d + 256 * half, p.D, p.vec, w[e]);
+#pragma unroll
+                for (int t = 0; t < TT; ++t) route_load8<T>(x[t], d + 256 * half, p.D, p.vec, v[t]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int e = 0; e < EW; ++e)
+#pragma unroll
+                        for (int t = 0; t < TT; ++t) part[e * TT + t] = fmaf(w[e][i], v[t][i], part[e * TT + t]);
             }
-        }
 #pragma unroll
-        for (int t = 0; t < kRouteTokens; ++t) {
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum[t] += __shfl_xor_sync(0xffffffffu, sum[t], o);
+            for (int i = 0; i < EW * TT; ++i) sum[i] += static_cast<double>(part[i]);
         }
+        reduce_lanes<EW * TT>(sum, lane);
+        if (!started) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA of the cluster runs
+        started = true;
         // Token t of the cluster is selected by CTA t.
-#pragma unroll
-        for (int t = 0; t < kRouteTokens; ++t)
-            if (lane == t) *cluster.map_shared_rank(&logits[e], t) = sum[t];
+        constexpr int kLanes = 32 / (EW * TT);
+        const int i = lane / kLanes, e = e0 + i / TT;
+        if (lane % kLanes == 0 && e < p.E) *cluster.map_shared_rank(&logits[e], i % TT) = sum[0];
     }
+    if (!started) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     cluster.sync();
     // One warp per token: softmax sums, then top_k rounds of a maximum over the keys.
     const int t = t0 + rank;
-    if (rank >= kRouteTokens || t >= p.T || warp != 0) return;
-    const double* l = logits;
+    if (rank >= TT || t >= p.T || warp != 0) return;
     double top = -INFINITY;
-    for (int e = lane; e < p.E; e += 32) top = fmax(top, l[e]);
+    for (int e = lane; e < p.E; e += 32) top = fmax(top, logits[e]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float total = 0.0f;
-    for (int e = lane; e < p.E; e += 32) total += expf(static_cast<float>(l[e] - top));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    float mine = 0.0f, chosen = 0.0f;
-    int my_id = 0;
-    unsigned long long taken = 0;  // this lane's experts that are chosen already, by e / 32
-    for (int k = 0; k < p.top_k; ++k) {
-        unsigned long long best = 0;
-        int at = p.E;
+    unsigned long long taken = 0, best = 0;  // this lane's chosen experts by e / 32; the largest key of the others
+    int at = p.E;                            // its expert, E if there is none
+    auto scan = [&]() {
+        best = 0;
+        at = p.E;
         for (int e = lane, i = 0; e < p.E; e += 32, ++i) {
-            const unsigned long long key = order_key(l[e]);
+            const unsigned long long key = order_key(logits[e]);
             if (!(taken >> i & 1) && (at == p.E || key > best)) best = key, at = e;
         }
-        int from = at;
+    };
+    scan();
+    float total = 0.0f;
+    for (int e = lane; e < p.E; e += 32) total += expf(static_cast<float>(logits[e] - top));
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
-            const int oe = __shfl_xor_sync(0xffffffffu, from, o);
-            if (oe < p.E && (from == p.E || other > best || (other == best && oe < from))) best = other, from = oe;
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    int my_id = 0;
+    for (int k = 0; k < p.top_k; ++k) {
+        // The largest upper half, the largest lower half among those, the lowest expert among those.
+        const bool any = at < p.E;
+        const unsigned hi = any ? static_cast<unsigned>(best >> 32) : 0u;
+        const unsigned high = __reduce_max_sync(0xffffffffu, hi);
+        const unsigned lo = any && hi == high ? static_cast<unsigned>(best) : 0u;
+        const unsigned low = __reduce_max_sync(0xffffffffu, lo);
+        const int from = __reduce_min_sync(0xffffffffu, any && hi == high && lo == low ? at : p.E);
+        if (lane == k) my_id = from;
+        if (any && at == from) {
+            taken |= 1ull << (at / 32);
+            scan();
         }
-        if (from == at && at < p.E) taken |= 1ull << (at / 32);
-        const float w = expf(static_cast<float>(l[from] - top)) / total;
-        chosen += w;
-        if (lane == k) mine = w, my_id = from;
     }
+    const float mine = lane < p.top_k ? expf(static_cast<float>(logits[my_id] - top)) / total : 0.0f;
+    float chosen = mine;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) chosen += __shfl_xor_sync(0xffffffffu, chosen, o);
     if (lane < p.top_k) {
-        const size_t at = static_cast<size_t>(t) * p.top_k + lane;
-        p.ids[at] = my_id;
-        p.weights[at] = p.renormalize ? mine / chosen : mine;
+        const size_t to = static_cast<size_t>(t) * p.top_k + lane;
+        p.ids[to] = my_id;
+        p.weights[to] = p.renormalize ? mine / chosen : mine;
     }
+}
+
+template <typename T, int EW, int TT>
+int launch_route(const RouteParams& p, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(ceil_div(p.T, TT)) * kRouteCluster, 1, 1);
+    cfg.blockDim = dim3(kMoeThreads, 1, 1);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, moe_route_kernel<T, EW, TT>, p) == cudaSuccess) return HGEMM_OK;
+    cudaGetLastError();
+    return HGEMM_ERR_CUDA;
+}
+
+// Few tokens: a cluster each (18 clusters fit the GPU at most), 2 experts a warp at a time.  More: 4 tokens a cluster, 4 experts.
+template <typename T>
+int run_route(const RouteParams& p, cudaStream_t stream) {
+    return p.T <= 16 ? launch_route<T, 2, 1>(p, stream) : launch_route<T, 4, 4>(p, stream);
 }
 
 // ---- grouping pairs by expert ------------------------------------------------------------
@@ -519,20 +579,8 @@ int hgemm_moe_route(const void* x, int x_dtype, long long ldx, const void* route
     if (int rc = hgw::current_device(&sms, &dev)) return rc;
     hgw::RouteParams p{x, router, T > 1 ? ldx : 0, T, D, E, top_k, renormalize != 0, false, ids, weights};
     p.vec = !hgw::misaligned(x, 16) && !hgw::misaligned(router, 16) && D % 8 == 0 && p.ldx % (16 / size) == 0;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(hgw::ceil_div(T, hgw::kRouteTokens)) * hgw::kRouteCluster, 1, 1);
-    cfg.blockDim = dim3(hgw::kMoeThreads, 1, 1);
-    cfg.stream = reinterpret_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = x_dtype == HGEMM_DTYPE_F32 ? cudaLaunchKernelEx(&cfg, hgw::moe_route_kernel<float>, p)
-                                                     : cudaLaunchKernelEx(&cfg, hgw::moe_route_kernel<__nv_bfloat16>, p);
-    if (e == cudaSuccess) return HGEMM_OK;
-    cudaGetLastError();
-    return HGEMM_ERR_CUDA;
+    const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    return x_dtype == HGEMM_DTYPE_F32 ? hgw::run_route<float>(p, s) : hgw::run_route<__nv_bfloat16>(p, s);
 }
 
 size_t hgemm_w4_moe_workspace_bytes(int T, int top_k, int F) {

@@ -179,6 +179,8 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_w4_kernel(const T* __r
     constexpr int kGroups = 128 / GROUP, kParts = GROUP / 32;
     const int lane = threadIdx.x & 31, g = lane / 4, t = lane & 3;
     const unsigned k_pairs = (k_blocks + 1) / 2, warps = gridDim.x * kQuantWarps;
+    pdl_trigger();
+    pdl_wait();
     for (unsigned item = blockIdx.x * kQuantWarps + threadIdx.x / 32; item < items; item += warps) {
         const unsigned block = item / k_pairs;  // row block of the whole stack
         const int kp = static_cast<int>(item - block * k_pairs);
@@ -308,6 +310,8 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_w4_kernel(const uint
     const int lane = threadIdx.x & 31, g = lane / 4, t = lane & 3;
     const unsigned warps = gridDim.x * kQuantWarps;
     const UnpackConstants constants;
+    pdl_trigger();
+    pdl_wait();
     for (unsigned item = blockIdx.x * kQuantWarps + threadIdx.x / 32; item < items; item += warps) {
         const unsigned block = item / k_blocks;
         const int kb = static_cast<int>(item - block * k_blocks);
@@ -385,9 +389,8 @@ int launch_quantize(const T* w, int count, int N, int K, uint8_t* q, uint32_t* s
     const size_t items = static_cast<size_t>(count) * rb * ceil_div(kb, 2);
     if (items > 0x7FFFFFFFu) return HGEMM_ERR_UNSUPPORTED;  // 2^31 x 2048 elements
     constexpr auto kernel = quantize_w4_kernel<T, ZERO, GROUP, VEC>;
-    kernel<<<one_wave<kernel>(items, sms, dev), kQuantThreads, 0, stream>>>(w, N, K, rb, kb, ceil_div(K, GROUP),
-                                                                           static_cast<unsigned>(items), q, scales, zeros);
-    return cudaGetLastError() == cudaSuccess ? HGEMM_OK : HGEMM_ERR_CUDA;
+    return launch<kernel>(dim3(one_wave<kernel>(items, sms, dev)), kQuantThreads, 1, 0, stream, w, N, K, rb, kb, ceil_div(K, GROUP),
+                          static_cast<unsigned>(items), q, scales, zeros);
 }
 
 template <typename T>
@@ -407,10 +410,8 @@ int launch_dequantize(const Weight& v, int count, int N, int K, T* w, int sms, i
     const size_t items = static_cast<size_t>(count) * v.row_blocks * v.k_blocks;
     if (items > 0x7FFFFFFFu) return HGEMM_ERR_UNSUPPORTED;
     constexpr auto kernel = dequantize_w4_kernel<T, ZERO, VEC>;
-    kernel<<<one_wave<kernel>(items, sms, dev), kQuantThreads, 0, stream>>>(v.q, v.scales, v.zeros, N, K, v.row_blocks, v.k_blocks,
-                                                                           v.groups, v.group_shift,
-                                                                           static_cast<unsigned>(items), w);
-    return cudaGetLastError() == cudaSuccess ? HGEMM_OK : HGEMM_ERR_CUDA;
+    return launch<kernel>(dim3(one_wave<kernel>(items, sms, dev)), kQuantThreads, 1, 0, stream, v.q, v.scales, v.zeros, N, K,
+                          v.row_blocks, v.k_blocks, v.groups, v.group_shift, static_cast<unsigned>(items), w);
 }
 
 template <typename T>

@@ -736,8 +736,8 @@ int resident_ctas(int dev, int threads, size_t bytes) {
 
 // Launches KERNEL with a cluster of `cluster` CTAs.  Programmatic dependent launch: the CTAs may start while the
 // stream's previous kernel ends; they touch global memory only after griddepcontrol.wait.
-template <auto KERNEL, typename Params>
-int launch(dim3 grid, int threads, int cluster, size_t smem, cudaStream_t stream, const Params& p) {
+template <auto KERNEL, typename... Args>
+int launch(dim3 grid, int threads, int cluster, size_t smem, cudaStream_t stream, const Args&... args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
@@ -752,7 +752,7 @@ int launch(dim3 grid, int threads, int cluster, size_t smem, cudaStream_t stream
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1 ? 2 : 1;
-    if (cudaLaunchKernelEx(&cfg, KERNEL, p) == cudaSuccess) return 0;
+    if (cudaLaunchKernelEx(&cfg, KERNEL, args...) == cudaSuccess) return 0;
     cudaGetLastError();
     return -4;  // HGEMM_ERR_CUDA
 }

@@ -18,7 +18,7 @@ from typing import NamedTuple
 import torch
 
 from ._lib import check
-from .gemm import _fn, _on_device, _stream_handle
+from .gemm import _fn, _get_device, _stream_handle
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 _GROUPS = (32, 64, 128)
@@ -49,46 +49,85 @@ def _dtype_code(name: str, t: torch.Tensor) -> int:
 
 
 def _check_weight(name: str, w: W4Weight, dev: int, count: int | None) -> None:
-    """Shapes, types and place of a weight's buffers; `count` experts, or one matrix (None)."""
+    """Types, sizes and place of a weight's buffers; `count` experts, or one matrix (None)."""
+    # A few cheap tests in the common case (this wrapper's host time adds to every launch of a small
+    # product); anything else takes the detailed ones, which raise the specific error.
+    q, s, z, n, k, group = w
+    if group in _GROUPS:
+        rb = (1 if count is None else count) * ((n + 15) // 16)
+        groups = rb * ((k + group - 1) // group) * 16
+        if (q.numel() == rb * ((k + 63) // 64) * 512 and s.numel() == groups and q.dtype is torch.uint8
+                and s.dtype is torch.bfloat16 and q.is_contiguous() and s.is_contiguous() and q.get_device() == dev >= 0
+                and s.get_device() == dev and (z is None or (z.numel() == groups and z.dtype is torch.uint8
+                                                             and z.is_contiguous() and z.get_device() == dev))):
+            return
+    _check_weight_in_detail(name, w, dev, count)
+
+
+def _check_weight_in_detail(name: str, w: W4Weight, dev: int, count: int | None) -> None:
     q, s, z, n, k, group = w
     if group not in _GROUPS:
         raise ValueError(f"{name}.group must be 32, 64 or 128, got {group}")
     rb, lead = -(-n // 16), () if count is None else (count,)
-    if q.dtype != torch.uint8 or q.shape != (*lead, rb, -(-k // 64), 512) or not q.is_contiguous():
-        raise ValueError(f"{name}.q must be a contiguous uint8 tensor of shape {(*lead, rb, -(-k // 64), 512)}")
+    shape = (*lead, rb, -(-k // 64), 512)
+    if q.dtype != torch.uint8 or q.shape != shape or not q.is_contiguous():
+        raise ValueError(f"{name}.q must be a contiguous uint8 tensor of shape {shape}")
     shape = (*lead, rb, -(-k // group), 8, 2)
     if s.dtype != torch.bfloat16 or s.shape != shape or not s.is_contiguous():
         raise ValueError(f"{name}.scales must be a contiguous bfloat16 tensor of shape {shape}")
     if z is not None and (z.dtype != torch.uint8 or z.shape != shape or not z.is_contiguous()):
         raise ValueError(f"{name}.zeros must be a contiguous uint8 tensor of shape {shape}")
-    if q.get_device() != dev or s.get_device() != dev or (z is not None and z.get_device() != dev):
-        raise ValueError(f"{name} must be on the same CUDA device as the other tensors (there is no CPU path)")
+    raise ValueError(f"{name} must be on the same CUDA device as the other tensors (there is no CPU path)")
 
 
-def _check_rows(name: str, x: torch.Tensor) -> int:
-    """A 2-D CUDA tensor with contiguous rows; its row stride in elements."""
-    if not x.is_cuda:
+def _check_rows(name: str, x: torch.Tensor) -> tuple[int, int, int]:
+    """Row stride (elements), type code and device index of a 2-D fp32 or bf16 CUDA tensor with contiguous rows."""
+    dev = x.get_device()
+    if dev < 0:
         raise ValueError(f"{name} must be on a CUDA device (there is no CPU path)")
-    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+    if x.dim() != 2:
         raise ValueError(f"{name} must be a 2-D tensor with contiguous, non-overlapping rows")
-    return x.stride(0)
+    ld, one = x.stride()
+    rows, columns = x.shape
+    if (columns > 1 and one != 1) or (rows > 1 and ld < columns):
+        raise ValueError(f"{name} must be a 2-D tensor with contiguous, non-overlapping rows")
+    dt = _DTYPES.get(x.dtype)
+    return ld, _dtype_code(name, x) if dt is None else dt, dev
 
 
-class _stream_of:
-    """torch's allocations inside belong to `stream` (the stream the kernels run on), so that
-    memory freed on another stream is not handed out while it is in use."""
+class _on:
+    """Device `dev` and, for torch's allocations, `stream` (the stream that the kernels run on: memory
+    freed on another one must not be handed out while it is in use) made current for a call."""
 
-    def __init__(self, stream: torch.cuda.Stream | None):
-        self.ctx = None if stream is None else torch.cuda.stream(stream)
+    def __init__(self, dev: int, stream: torch.cuda.Stream | None):
+        self.parts = [torch.cuda.device(dev)] if stream is None else [torch.cuda.device(dev), torch.cuda.stream(stream)]
 
     def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
+        for part in self.parts:
+            part.__enter__()
 
     def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
+        for part in reversed(self.parts):
+            part.__exit__(*exc)
         return False
+
+
+class _Nothing:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *exc):
+        return False
+
+
+_nothing = _Nothing()
+
+
+def _context(dev: int, stream: torch.cuda.Stream | None):
+    """A context for a call on `dev` and `stream`; none where both are current already."""
+    if stream is None and _get_device is not None and _get_device() == dev:
+        return _nothing
+    return _on(dev, stream)
 
 
 def w4_pack(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, *, group: int) -> W4Weight:
@@ -134,10 +173,10 @@ def quantize_w4(w: torch.Tensor, group: int = 128, zero_point: bool = False,
         raise ValueError(f"group must be 32, 64 or 128, got {group}")
     *lead, n, k = w.shape
     rb, dev = -(-n // 16), w.get_device()
-    with _on_device(dev), _stream_of(stream):
-        q = torch.empty((*lead, rb, -(-k // 64), 512), dtype=torch.uint8, device=w.device)
-        scales = torch.empty((*lead, rb, -(-k // group), 8, 2), dtype=torch.bfloat16, device=w.device)
-        zeros = torch.empty(scales.shape, dtype=torch.uint8, device=w.device) if zero_point else None
+    with _context(dev, stream):
+        q = w.new_empty((*lead, rb, -(-k // 64), 512), dtype=torch.uint8)
+        scales = w.new_empty((*lead, rb, -(-k // group), 8, 2), dtype=torch.bfloat16)
+        zeros = w.new_empty(scales.shape, dtype=torch.uint8) if zero_point else None
         rc = _fn("hgemm_quantize_w4")(w.data_ptr(), dt, lead[0] if lead else 1, n, k, group, q.data_ptr(),
                                       scales.data_ptr(), zeros.data_ptr() if zero_point else None,
                                       _stream_handle(stream, dev))
@@ -148,14 +187,14 @@ def quantize_w4(w: torch.Tensor, group: int = 128, zero_point: bool = False,
 def dequantize_w4(w: W4Weight, dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None,
                   stream: torch.cuda.Stream | None = None) -> torch.Tensor:
     """The values of a 4-bit weight, (N, K) or (E, N, K): (code - zero) * scale, rounded once."""
-    if not w.q.is_cuda:
-        raise ValueError("w must be on a CUDA device (there is no CPU path)")
     dev, count = w.q.get_device(), w.experts
+    if dev < 0:
+        raise ValueError("w must be on a CUDA device (there is no CPU path)")
     _check_weight("w", w, dev, count)
     shape = (w.n, w.k) if count is None else (count, w.n, w.k)
-    with _on_device(dev), _stream_of(stream):
+    with _context(dev, stream):
         if out is None:
-            out = torch.empty(shape, dtype=dtype, device=w.q.device)
+            out = w.q.new_empty(shape, dtype=dtype)
         elif out.shape != shape or out.dtype != dtype or not out.is_contiguous() or out.get_device() != dev:
             raise ValueError(f"out must be a contiguous {dtype} tensor of shape {shape} on w's device")
         rc = _fn("hgemm_dequantize_w4")(w.q.data_ptr(), w.scales.data_ptr(), None if w.zeros is None else w.zeros.data_ptr(),
@@ -169,15 +208,14 @@ def w4_gemm_tn(x: torch.Tensor, w: W4Weight, out: torch.Tensor | None = None, *,
                stream: torch.cuda.Stream | None = None) -> torch.Tensor:
     """y[M,N] = x[M,K] @ W[N,K]^T for a few rows of x (fp32 or bf16, rows may be strided); y has x's
     type, sums are fp32 (hgemm_w4_gemm_tn).  For many rows use dequantize_w4 and a matrix product."""
-    ldx = _check_rows("x", x)
-    dt, dev = _dtype_code("x", x), x.get_device()
+    ldx, dt, dev = _check_rows("x", x)
     _check_weight("w", w, dev, None)
     m, k = x.shape
     if k != w.k:
         raise ValueError(f"K mismatch: x is {tuple(x.shape)}, w is {w.n} x {w.k}")
-    with _on_device(dev), _stream_of(stream):
+    with _context(dev, stream):
         if out is None:
-            out = torch.empty((m, w.n), dtype=x.dtype, device=x.device)
+            out = x.new_empty((m, w.n))
         elif out.shape != (m, w.n) or out.dtype != x.dtype or not out.is_contiguous() or out.get_device() != dev:
             raise ValueError("out must be a contiguous (M, N) tensor of x's type on x's device")
         rc = _fn("hgemm_w4_gemm_tn")(x.data_ptr(), dt, ldx, w.q.data_ptr(), w.scales.data_ptr(),
@@ -193,17 +231,16 @@ def moe_route(x: torch.Tensor, router: torch.Tensor, top_k: int, *, renormalize:
     """The router of a mixture of experts (hgemm_moe_route): softmax(x[T,D] @ router[E,D]^T) and per
     token the top_k largest: ids (T, top_k) int32, largest first, and their probabilities (T,
     top_k) float32, which add up to 1 with renormalize.  E <= 1024, top_k <= 16."""
-    ldx = _check_rows("x", x)
-    dt, dev = _dtype_code("x", x), x.get_device()
+    ldx, dt, dev = _check_rows("x", x)
     if router.dtype != x.dtype or router.dim() != 2 or not router.is_contiguous() or router.get_device() != dev:
         raise ValueError("router must be a contiguous (E, D) tensor of x's type on x's device")
     t, d = x.shape
     e = router.shape[0]
     if router.shape[1] != d:
         raise ValueError(f"D mismatch: x is {tuple(x.shape)}, router is {tuple(router.shape)}")
-    with _on_device(dev), _stream_of(stream):
-        ids = torch.empty((t, max(top_k, 0)), dtype=torch.int32, device=x.device)
-        weights = torch.empty((t, max(top_k, 0)), dtype=torch.float32, device=x.device)
+    with _context(dev, stream):
+        ids = x.new_empty((t, max(top_k, 0)), dtype=torch.int32)
+        weights = x.new_empty((t, max(top_k, 0)), dtype=torch.float32)
         rc = _fn("hgemm_moe_route")(x.data_ptr(), dt, ldx, router.data_ptr(), t, d, e, top_k, bool(renormalize),
                                     ids.data_ptr(), weights.data_ptr(), _stream_handle(stream, dev))
     if rc:
@@ -220,8 +257,7 @@ def w4_moe(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate: W4We
     them (ids outside [0, E) add nothing), gate and up (E, F, D), down (E, D, F).  workspace:
     hgemm_w4_moe_workspace_bytes(T, top_k, F) bytes that no other running call uses, else
     allocated by torch."""
-    ldx = _check_rows("x", x)
-    dt, dev = _dtype_code("x", x), x.get_device()
+    ldx, dt, dev = _check_rows("x", x)
     t, d = x.shape
     e, f = gate.experts, gate.n
     if e is None:
@@ -238,13 +274,13 @@ def w4_moe(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate: W4We
     if (weights.dtype != torch.float32 or weights.shape != ids.shape or not weights.is_contiguous()
             or weights.get_device() != dev):
         raise ValueError("weights must be a contiguous (T, top_k) float32 tensor on x's device")
-    with _on_device(dev), _stream_of(stream):
+    with _context(dev, stream):
         if out is None:
-            out = torch.empty((t, d), dtype=x.dtype, device=x.device)
+            out = x.new_empty((t, d))
         elif out.shape != (t, d) or out.dtype != x.dtype or not out.is_contiguous() or out.get_device() != dev:
             raise ValueError("out must be a contiguous (T, D) tensor of x's type on x's device")
         if workspace is None:
-            workspace = torch.empty(_fn("hgemm_w4_moe_workspace_bytes")(t, top_k, f), dtype=torch.uint8, device=x.device)
+            workspace = x.new_empty(_fn("hgemm_w4_moe_workspace_bytes")(t, top_k, f), dtype=torch.uint8)
         elif workspace.get_device() != dev or not workspace.is_contiguous():
             raise ValueError("workspace must be a contiguous tensor on x's device")
         # Three hgemm_w4_weight: q, scales, zeros, group.
