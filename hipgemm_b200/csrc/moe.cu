@@ -27,13 +27,15 @@ constexpr int kMaxSegments = kMaxPairs;
 
 // ---- router -----------------------------------------------------------------------------
 //
-// A cluster of 8 CTAs takes TT tokens; its 64 warps split the experts, EW at a time, so that a
-// load of x serves EW experts and one of the router TT tokens.  Sixteen products a lane are summed
-// in fp32 and then added in 64 bits, so that experts whose logits are close are ordered as the
-// exact logits are.  The logits go to the CTA that selects the token's experts over distributed
-// shared memory.
+// A cluster of 8 CTAs takes TT tokens; its warps, in pairs that take half of D each, split the
+// experts, EW at a time, so that a load of x serves EW experts and one of the router TT tokens.
+// Sixteen products a lane are summed in fp32 and then added in 64 bits, so that experts whose logits
+// are close are ordered as the exact logits are.  The logits go to the CTA that selects the
+// token's experts over distributed shared memory.  Bound by the latency of the router's loads
+// (each cluster reads all of it from L2): hence 16 warps, and two loads of each row at a time.
 
 constexpr int kRouteCluster = 8;
+constexpr int kRouteWarps = 8;
 
 struct RouteParams {
     const void* x;
@@ -45,31 +47,33 @@ struct RouteParams {
     float* weights;
 };
 
-// 8 elements of a row; zeros at and past `len`.
+// A lane's 16 bytes of a row: 4 fp32 or 8 bf16 from `at` on; zeros at and past `len`.
 template <typename T>
-__device__ __forceinline__ void route_load8(const T* row, int at, int len, bool vec, float (&v)[8]) {
-    if (vec) {
-        if (at >= len) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-        } else if constexpr (sizeof(T) == 4) {
-            const float4 a = __ldg(reinterpret_cast<const float4*>(row + at));
-            const float4 b = __ldg(reinterpret_cast<const float4*>(row + at) + 1);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+struct RouteLoad {
+    static constexpr int kElements = 16 / sizeof(T);
+    uint4 v;
+    __device__ __forceinline__ void load_full(const T* row, int at) { v = __ldg(reinterpret_cast<const uint4*>(row + at)); }
+    __device__ __forceinline__ void load(const T* row, int at, int len, bool vec) {
+        v = make_uint4(0u, 0u, 0u, 0u);
+        if (vec) {
+            if (at < len) v = __ldg(reinterpret_cast<const uint4*>(row + at));
         } else {
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + at));
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+            uint32_t e[kElements];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[2 * i] = bf16_lo(w[i]), v[2 * i + 1] = bf16_hi(w[i]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if constexpr (sizeof(T) == 4) v[i] = at + i < len ? row[at + i] : 0.0f;
-            else v[i] = at + i < len ? __bfloat162float(row[at + i]) : 0.0f;
+            for (int i = 0; i < kElements; ++i) {
+                if constexpr (sizeof(T) == 4) e[i] = at + i < len ? __float_as_uint(row[at + i]) : 0u;
+                else e[i] = at + i < len ? __ldg(reinterpret_cast<const unsigned short*>(row + at + i)) : 0u;
+            }
+            if constexpr (sizeof(T) == 4) v = make_uint4(e[0], e[1], e[2], e[3]);
+            else v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
         }
     }
-}
+    __device__ __forceinline__ float element(int i) const {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else return i & 1 ? bf16_hi(w[i / 2]) : bf16_lo(w[i / 2]);
+    }
+};
 
 // A key that orders as the numbers do, NaN below everything.
 __device__ __forceinline__ unsigned long long order_key(double v) {
@@ -78,28 +82,30 @@ __device__ __forceinline__ unsigned long long order_key(double v) {
     return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
 
-// Sums v[i] over the lanes: afterwards v[0] of lane l is the sum of v[l / (32 / N)].
-template <int N>
-__device__ __forceinline__ void reduce_lanes(double (&v)[N], int lane) {
+// Sums v[i], i < N, over the lanes: afterwards v[0] of lane l is the sum of v[l / (32 / N)].  (A recursion over
+// N, so that every index is known and v stays in registers.)
+template <int N, int O = 16, int M>
+__device__ __forceinline__ void reduce_lanes(double (&v)[M], int lane) {
+    if constexpr (O > 0) {
+        if constexpr (N > 1) {
+            const bool upper = (lane & O) != 0;
 #pragma unroll
-    for (int o = 16, n = N; o > 0; o >>= 1) {
-        if (n > 1) {
-            const bool upper = (lane & o) != 0;
-            n /= 2;
-#pragma unroll
-            for (int i = 0; i < n; ++i) {
-                const double keep = upper ? v[n + i] : v[i], give = upper ? v[i] : v[n + i];
-                v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+            for (int i = 0; i < N / 2; ++i) {
+                const double keep = upper ? v[N / 2 + i] : v[i], give = upper ? v[i] : v[N / 2 + i];
+                v[i] = keep + __shfl_xor_sync(0xffffffffu, give, O);
             }
+            reduce_lanes<N / 2, O / 2>(v, lane);
         } else {
-            v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+            v[0] += __shfl_xor_sync(0xffffffffu, v[0], O);
+            reduce_lanes<1, O / 2>(v, lane);
         }
     }
 }
 
 template <typename T, int EW, int TT>
-__global__ void __launch_bounds__(kMoeThreads) __cluster_dims__(kRouteCluster, 1, 1) moe_route_kernel(const RouteParams p) {
-    __shared__ double logits[kMaxExperts];  // of the token that this CTA selects for
+__global__ void __launch_bounds__(kRouteWarps * 32, 2) __cluster_dims__(kRouteCluster, 1, 1) moe_route_kernel(const RouteParams p) {
+    __shared__ double halves[2][kMaxExperts];  // logits of the token that this CTA selects for, by half of D
+    double* logits = halves[0];
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = static_cast<int>(cluster.block_rank());
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
@@ -111,27 +117,46 @@ __global__ void __launch_bounds__(kMoeThreads) __cluster_dims__(kRouteCluster, 1
     const T* x[TT];
 #pragma unroll
     for (int t = 0; t < TT; ++t) x[t] = static_cast<const T*>(p.x) + min(t0 + t, p.T - 1) * p.ldx;
+    constexpr int kChunk = 32 * RouteLoad<T>::kElements, kFlush = 16 / RouteLoad<T>::kElements;  // chunks between additions in 64 bits
+    const int half = warp & 1, middle = ceil_div(p.D, 2 * kChunk) * kChunk, d1 = half ? p.D : min(middle, p.D);
     bool started = false;
-    for (int e0 = (rank * kMoeWarps + warp) * EW; e0 < p.E; e0 += kRouteCluster * kMoeWarps * EW) {
+    for (int e0 = (rank * kRouteWarps + warp) / 2 * EW; e0 < p.E; e0 += kRouteCluster * kRouteWarps / 2 * EW) {
         const T* r[EW];
 #pragma unroll
         for (int e = 0; e < EW; ++e) r[e] = static_cast<const T*>(p.router) + static_cast<size_t>(min(e0 + e, p.E - 1)) * p.D;
         double sum[EW * TT] = {};
-        for (int d = lane * 8; d < p.D; d += 512) {
+        for (int d = half * middle; d < d1; d += kFlush * kChunk) {
             float part[EW * TT] = {};
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                float w[EW][8], v[TT][8];
+            for (int c = 0; c < kFlush; c += 2) {
+                RouteLoad<T> w[2][EW], v[2][TT];
+                const int at = d + c * kChunk + lane * RouteLoad<T>::kElements;
+                if (p.vec && d + (c + 2) * kChunk <= d1) {  // a branch for all loads together, so that they are in flight together
 #pragma unroll
-                for (int e = 0; e < EW; ++e) route_load8<T>(r[e], d + 256 * half, p.D, p.vec, w[e]);
+                    for (int u = 0; u < 2; ++u) {
 #pragma unroll
-                for (int t = 0; t < TT; ++t) route_load8<T>(x[t], d + 256 * half, p.D, p.vec, v[t]);
+                        for (int e = 0; e < EW; ++e) w[u][e].load_full(r[e], at + u * kChunk);
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
+                        for (int t = 0; t < TT; ++t) v[u][t].load_full(x[t], at + u * kChunk);
+                    }
+                } else {
 #pragma unroll
-                    for (int e = 0; e < EW; ++e)
+                    for (int u = 0; u < 2; ++u) {
 #pragma unroll
-                        for (int t = 0; t < TT; ++t) part[e * TT + t] = fmaf(w[e][i], v[t][i], part[e * TT + t]);
+                        for (int e = 0; e < EW; ++e) w[u][e].load(r[e], at + u * kChunk, d1, p.vec);
+#pragma unroll
+                        for (int t = 0; t < TT; ++t) v[u][t].load(x[t], at + u * kChunk, d1, p.vec);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < RouteLoad<T>::kElements; ++i)
+#pragma unroll
+                        for (int e = 0; e < EW; ++e)
+#pragma unroll
+                            for (int t = 0; t < TT; ++t)
+                                part[e * TT + t] = fmaf(w[u][e].element(i), v[u][t].element(i), part[e * TT + t]);
             }
 #pragma unroll
             for (int i = 0; i < EW * TT; ++i) sum[i] += static_cast<double>(part[i]);
@@ -142,7 +167,7 @@ __global__ void __launch_bounds__(kMoeThreads) __cluster_dims__(kRouteCluster, 1
         // Token t of the cluster is selected by CTA t.
         constexpr int kLanes = 32 / (EW * TT);
         const int i = lane / kLanes, e = e0 + i / TT;
-        if (lane % kLanes == 0 && e < p.E) *cluster.map_shared_rank(&logits[e], i % TT) = sum[0];
+        if (lane % kLanes == 0 && e < p.E) *cluster.map_shared_rank(&halves[half][e], i % TT) = sum[0];
     }
     if (!started) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     cluster.sync();
@@ -150,7 +175,10 @@ __global__ void __launch_bounds__(kMoeThreads) __cluster_dims__(kRouteCluster, 1
     const int t = t0 + rank;
     if (rank >= TT || t >= p.T || warp != 0) return;
     double top = -INFINITY;
-    for (int e = lane; e < p.E; e += 32) top = fmax(top, logits[e]);
+    for (int e = lane; e < p.E; e += 32) {
+        logits[e] += halves[1][e];
+        top = fmax(top, logits[e]);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
     unsigned long long taken = 0, best = 0;  // this lane's chosen experts by e / 32; the largest key of the others
@@ -168,6 +196,7 @@ __global__ void __launch_bounds__(kMoeThreads) __cluster_dims__(kRouteCluster, 1
     for (int e = lane; e < p.E; e += 32) total += expf(static_cast<float>(logits[e] - top));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    __syncwarp();
     int my_id = 0;
     for (int k = 0; k < p.top_k; ++k) {
         // The largest upper half, the largest lower half among those, the lowest expert among those.
@@ -198,7 +227,7 @@ template <typename T, int EW, int TT>
 int launch_route(const RouteParams& p, cudaStream_t stream) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(ceil_div(p.T, TT)) * kRouteCluster, 1, 1);
-    cfg.blockDim = dim3(kMoeThreads, 1, 1);
+    cfg.blockDim = dim3(kRouteWarps * 32, 1, 1);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
