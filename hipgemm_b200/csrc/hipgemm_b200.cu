@@ -674,6 +674,27 @@ int run_gemm_mx(const void* A, const void* B, void* C, int M, int N, int K, cons
 }  // namespace
 }  // namespace hg
 
+namespace hg {
+
+// The status word's address on the current device, for kernels of other translation units; null on
+// failure.  Looked up once per device.
+uint32_t* status_word(int dev) {
+    static std::atomic<uint32_t*> known[kMaxDevices];
+    uint32_t* p = known[dev].load(std::memory_order_relaxed);
+    if (!p) {
+        void* address = nullptr;
+        if (cudaGetSymbolAddress(&address, g_status) != cudaSuccess) {
+            cudaGetLastError();
+            return nullptr;
+        }
+        p = static_cast<uint32_t*>(address);
+        known[dev].store(p, std::memory_order_relaxed);
+    }
+    return p;
+}
+
+}  // namespace hg
+
 extern "C" {
 
 int hgemm_fp8_tn_mx(const void* A, const void* B, void* C, int M, int N, int K, const void* SFA, const void* SFB,

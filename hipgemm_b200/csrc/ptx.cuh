@@ -15,11 +15,14 @@
 
 namespace hg {
 
+#ifndef HG_PTX_WITHOUT_STATUS
 // Device-global status word: 0 while healthy, else the code of the first bounded
 // wait that expired (site code in the low byte, role in the next).  Read and cleared
 // by hgemm_device_status().  Defined here: exactly one translation unit of the
-// library includes this header.
+// library includes this header without HG_PTX_WITHOUT_STATUS; others take its address
+// from hg::status_word().
 __device__ uint32_t g_status = 0;
+#endif
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -97,6 +100,7 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t par
     return ok != 0;
 }
 
+#ifndef HG_PTX_WITHOUT_STATUS
 __device__ __forceinline__ void record_error(uint32_t code) { atomicCAS(&g_status, 0u, code); }
 
 // Bounded wait for the phase of parity `parity` to complete.  Returns false when the
@@ -122,6 +126,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
         }
     }
 }
+#endif
 
 // Spin for about `ns` nanoseconds (used only on the abort path to let copies land).
 __device__ __forceinline__ void sleep_ns_bounded(uint64_t ns) {

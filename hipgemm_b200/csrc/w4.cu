@@ -662,7 +662,7 @@ struct RowsPlan {
 
 // Clusters of `split` CTAs, one an SM, that the device keeps resident: a cluster lies in one GPC, so that fewer
 // than SMs / split fit (B200: 74 of 2, 33 of 4).  Every instance of the kernel fills an SM alike.
-inline int resident_clusters(int split, int sms, int dev) {
+int resident_clusters(int split, int sms, int dev) {
     static std::atomic<int> known[kMaxDevices][4];
     if (split == 1) return sms;
     std::atomic<int>& slot = known[dev][split / 2];
@@ -739,6 +739,10 @@ bool run_rows(const LinearParams& p, int sms, int dev, cudaStream_t stream, int*
     return true;
 }
 
+// w4_tc.cu
+int run_tc(const void* x, long long ldx, void* y, int M, int N, int K, const Weight& w, int group, int sms, int dev,
+           cudaStream_t stream);
+
 template <typename T, int GROUP, bool ZERO>
 int run_linear(const LinearParams& p, int sms, int dev, cudaStream_t stream) {
     int rc = 0;
@@ -746,6 +750,9 @@ int run_linear(const LinearParams& p, int sms, int dev, cudaStream_t stream) {
     if constexpr (sizeof(T) == 4) {
         return launch_linear<T, 2, 1, 3, GROUP, ZERO, 4>(p, sms, dev, stream);
     } else {
+        // Measured at 8192 x 8192 (28672 x 8192): 16 rows 14.8 (46.4) us here and 14.5 (43.2) there, but 5.6 and 7.4 at 4096 x 4096;
+        // 17 rows 28.5 (86.4) and 16.7 (51.7); 64 rows 44.3 (153) and 21.7 (68.2).
+        if (p.M > 16 && p.vec) return run_tc(p.x, p.ldx, p.y, p.M, p.N, p.K, p.w, GROUP, sms, dev, stream);
         if (p.M <= 8) return launch_linear<T, 2, 1, 3, GROUP, ZERO, 8>(p, sms, dev, stream);
         if (p.M <= 16) return launch_linear<T, 2, 2, 3, GROUP, ZERO, 4>(p, sms, dev, stream);
         return launch_linear<T, 2, 4, 3, GROUP, ZERO, 4>(p, sms, dev, stream);

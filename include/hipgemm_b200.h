@@ -187,7 +187,8 @@ int hgemm_config_resident_ctas(int config);
  * bounded wait has expired since the last call, else the code of the first one,
  * role << 8 | site: 0x0101 producer (stage free), 0x0201 / 0x0202 / 0x0203 MMA issuer
  * (accumulator free, stage full, drain), 0x0301 epilogue (accumulator full), 0x0303
- * split-K epilogue (peers' partial columns in). */
+ * split-K epilogue (peers' partial columns in); 0x04xx to 0x07xx the 4-bit product's flush,
+ * unpacking, x copy and MMA roles. */
 int hgemm_device_status(uint32_t* status_out);
 
 /* Test hook: 1 if the library's stream-K workspace pool exists on `device` (it is created
