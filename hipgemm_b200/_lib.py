@@ -74,7 +74,7 @@ _SIGNATURES = {
     "hgemm_moe_route": (_i, [_vp, _i, ctypes.c_longlong, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp]),
     "hgemm_w4_moe": (_i, [_vp, _i, ctypes.c_longlong, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp,
                           ctypes.c_size_t, _vp]),
-    "hgemm_w4_moe_workspace_bytes": (ctypes.c_size_t, [_i, _i, _i]),
+    "hgemm_w4_moe_workspace_bytes": (ctypes.c_size_t, [_i, _i, _i, _i]),
     "hgemm_num_configs": (_i, []),
     "hgemm_config_resident_ctas": (_i, [_i]),
     "hgemm_config_name": (ctypes.c_char_p, [_i]),

@@ -6,6 +6,7 @@
 //
 // Both products of the experts read each reached expert's codes once for all the tokens that are
 // sent to it: (token, expert) pairs are grouped by expert into segments of up to 8 NT columns.
+// A third, small kernel adds up a token's experts, in the order of its ids.
 #include <cooperative_groups.h>
 
 #include <atomic>
@@ -259,25 +260,55 @@ struct PairLists {
     int n_segments;
 };
 
-// Fills the lists from ids (T x top_k), T * top_k <= kMaxPairs.  A pair counts when its id is in
-// [0, E) and its token does not have the same id at an earlier place (the weights of such pairs
-// are added to the first one's).  Within an expert pairs keep their order, so that the sums'
-// order, and with it every bit of the result, depends on the inputs alone.  All threads call it.
+// Whether pair p counts: its id is in [0, E) and its token does not have the same id at an earlier place (the
+// weights of such pairs are added to the first one's).  The id, or -1.
+__device__ __forceinline__ int counted_id(const int* ids, int p, int top_k, int E) {
+    int id = ids[p];
+    if (id < 0 || id >= E) return -1;
+    for (int q = p / top_k * top_k; q < p; ++q)
+        if (ids[q] == id) return -1;
+    return id;
+}
+
+// Fills the lists from ids (T x top_k), T * top_k <= kMaxPairs.  Within an expert pairs keep their order, and so
+// do the segments: the result's bits depend on the inputs alone.  All threads call it.
 __device__ void build_lists(PairLists& s, const int* ids, int T, int top_k, int E, int columns) {
-    const int pairs = T * top_k;
+    const int pairs = T * top_k, lane = threadIdx.x & 31;
+    __shared__ int done;
+    if (threadIdx.x < 32) {
+        // Up to 32 pairs, and no expert with more than a segment: all in one warp's registers.
+        bool ok = false;
+        if (pairs <= 32) {
+            const int id = lane < pairs ? counted_id(ids, lane, top_k, E) : -1;
+            const unsigned same = __match_any_sync(0xffffffffu, id), below = (1u << lane) - 1u;
+            const int count = id >= 0 ? __popc(same) : 0, rank = __popc(same & below);
+            ok = __all_sync(0xffffffffu, count <= columns);
+            if (ok) {
+                const bool leads = id >= 0 && rank == 0;
+                const unsigned leaders = __ballot_sync(0xffffffffu, leads);
+                int first = leads ? count : 0;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int up = __shfl_up_sync(0xffffffffu, first, o);
+                    if (lane >= o) first += up;
+                }
+                first -= leads ? count : 0;
+                if (leads)
+                    s.segments[__popc(leaders & below)] = {static_cast<short>(id), static_cast<short>(first), static_cast<short>(count), 0};
+                first = __shfl_sync(0xffffffffu, first, __ffs(same) - 1);
+                if (id >= 0) s.order[first + rank] = static_cast<short>(lane);
+                if (lane == 0) s.n_segments = __popc(leaders);
+            }
+        }
+        if (lane == 0) done = ok;
+    }
+    __syncthreads();
+    if (done) return;
     for (int e = threadIdx.x; e < E; e += kMoeThreads) s.count[e] = 0;
     __syncthreads();
     if (threadIdx.x < 32) {
-        const int lane = threadIdx.x;
         for (int p0 = 0; p0 < pairs; p0 += 32) {
-            const int p = p0 + lane;
-            int id = -1;
-            if (p < pairs) {
-                id = ids[p];
-                if (id < 0 || id >= E) id = -1;
-                for (int q = p / top_k * top_k; q < p && id >= 0; ++q)
-                    if (ids[q] == id) id = -1;
-            }
+            const int p = p0 + lane, id = p < pairs ? counted_id(ids, p, top_k, E) : -1;
             const unsigned same = __match_any_sync(0xffffffffu, id);
             const int before = __popc(same & ((1u << lane) - 1u)), base = id >= 0 ? s.count[id] : 0;
             __syncwarp();
@@ -311,12 +342,15 @@ __device__ void build_lists(PairLists& s, const int* ids, int T, int top_k, int 
     __syncthreads();
 }
 
-// ---- experts: h = silu(gate x) * (up x) ------------------------------------------------------
+// ---- the experts' products ----------------------------------------------------------------------
 //
-// A persistent grid over (segment, RH row blocks of F); the CTA's warps split D.  For bf16 x, h is
-// kept as two bf16 whose sum has 16 significant bits or more: twice the matrix instructions in
-// the product with down, and no rounding to 8 bits between the two products, which would add as
-// much error as the output's own rounding.  For fp32 x it is kept in fp32.
+// A persistent grid over units: a segment's columns times 8 / WK groups of rows.  A group is RH row
+// blocks (of gate and of up, or of down); WK warps split its K, and their sums are joined in shared
+// memory in a fixed order.
+//
+// h = silu(gate x) * (up x) is kept, for bf16 x, as two bf16 whose sum has 16 significant bits or more: twice
+// the matrix instructions in the product with down, and no rounding to 8 bits between the two
+// products, which would add as much error as the output's own rounding.  For fp32 x it is kept in fp32.
 
 struct ExpertParams {
     const void* x;
@@ -329,85 +363,10 @@ struct ExpertParams {
     void* h;                // rows of h_stride elements by pair: fp32, or upper bf16 and h_low elements on the lower ones
     int h_stride;           // F rounded up to whole row blocks
     long long h_low;
+    float* y;               // rows of y_stride by pair: down's products
+    int y_stride;           // D rounded up to whole row blocks
     void* out;
 };
-
-template <typename T, int RH, int NT, int STAGES, int GROUP, bool ZERO>
-struct GateUpShape {
-    using Product = WarpProduct<2 * RH, NT, STAGES, GROUP, ZERO, RowSource<T>>;
-    static constexpr int kOut = 2 * RH * NT * 128;
-    static constexpr int kRings = kMoeWarps * Product::kWarpBytes, kSmem = kRings + kMoeWarps * kOut * 4;
-};
-
-template <typename T, int RH, int NT, int STAGES, int GROUP, bool ZERO>
-__global__ void __launch_bounds__(kMoeThreads) moe_gate_up_kernel(const ExpertParams p) {
-    using Shape = GateUpShape<T, RH, NT, STAGES, GROUP, ZERO>;
-    constexpr int kOut = Shape::kOut;
-    extern __shared__ __align__(16) uint8_t smem[];  // the warps' rings, then their sums
-    float* partial = reinterpret_cast<float*>(smem + Shape::kRings);
-    __shared__ PairLists lists;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-    pdl_trigger();
-    pdl_wait();
-    build_lists(lists, p.ids, p.T, p.top_k, p.E, 8 * NT);
-    const int chunks = (p.gate.row_blocks + RH - 1) / RH, units = lists.n_segments * chunks;
-    const int steps = ceil_div(p.gate.k_blocks, 2), s0 = steps * warp / kMoeWarps, s1 = steps * (warp + 1) / kMoeWarps;
-    for (int u = blockIdx.x; u < units; u += gridDim.x) {
-        const int seg = u / chunks, block0 = (u - seg * chunks) * RH;
-        const Segment sg = lists.segments[seg];
-        typename Shape::Product product;
-#pragma unroll
-        for (int r = 0; r < RH; ++r) {
-            const int block = min(block0 + r, p.gate.row_blocks - 1);
-            product.set_rows(r, p.gate, sg.expert, block, lane);
-            product.set_rows(RH + r, p.up, sg.expert, block, lane);
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int pair = lists.order[sg.first + min(8 * n + lane / 4, sg.columns - 1)], k = 8 * (lane & 3);
-            product.x[n] = {static_cast<const T*>(p.x) + static_cast<long long>(pair / p.top_k) * p.ldx + k, p.D - k, p.vec};
-        }
-        product.set_columns(p.vec ? p.D : 0);
-        float acc[2 * RH][NT][4] = {};
-        product.run(smem + warp * Shape::Product::kWarpBytes, s0, s1, lane, acc);
-#pragma unroll
-        for (int r = 0; r < 2 * RH; ++r)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) partial[warp * kOut + ((r * NT + n) * 4 + i) * 32 + lane] = acc[r][n][i];
-        __syncthreads();
-        for (int i = threadIdx.x; i < kOut / 2; i += kMoeThreads) {
-            float g = 0.0f, v = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kMoeWarps; ++w) {
-                g += partial[w * kOut + i];
-                v += partial[w * kOut + kOut / 2 + i];
-            }
-            const int l = i & 31, f = (i >> 5) & 3, n = (i >> 7) % NT, r = (i >> 7) / NT;
-            const int row = (block0 + r) * 16 + l / 4 + 8 * (f >> 1), col = 8 * n + 2 * (l & 3) + (f & 1);
-            if (row < p.h_stride && col < sg.columns) {
-                // Rows past F (up to the row block's end) are zeros, which the next product may read.
-                const float h = row < p.F ? g / (1.0f + expf(-g)) * v : 0.0f;
-                const size_t at = static_cast<size_t>(lists.order[sg.first + col]) * p.h_stride + row;
-                if constexpr (sizeof(T) == 4) {
-                    static_cast<float*>(p.h)[at] = h;
-                } else {
-                    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.h) + at;
-                    dst[0] = __ushort_as_bfloat16(static_cast<unsigned short>(__float_as_uint(h) >> 16));
-                    dst[p.h_low] = __float2bfloat16_rn(after_bf16(h));
-                }
-            }
-        }
-        __syncthreads();
-    }
-}
-
-// ---- experts: out = sum of the weighted products with down -------------------------------------
-//
-// A cluster takes R row blocks of D for all pairs: the list of (segment, K block) steps is split
-// over its warps, and each warp adds its part of a segment, times the router's weight, to its own
-// sums of every token.  The warps' sums, then the CTAs', are joined in a fixed order.
 
 // Rows of h as two bf16 terms, 16-byte aligned and a multiple of 16 long.
 struct SplitSource {
@@ -449,97 +408,133 @@ struct SplitSource {
     }
 };
 
-template <typename T, int R, int NT, int STAGES, int GROUP, bool ZERO>
-struct DownShape {
-    using Source = std::conditional_t<sizeof(T) == 4, RowSource<float>, SplitSource>;
-    using Product = WarpProduct<R, NT, STAGES, GROUP, ZERO, Source>;
-    static constexpr int kRows = 16 * R;
-    static constexpr int kStride = kRows + 8;  // a token's sums: columns 2 t, 2 t + 1 of a warp's store to distinct banks
-    static constexpr int kRings = kMoeWarps * Product::kWarpBytes;
-    static constexpr int smem(int tokens) { return kRings + kMoeWarps * tokens * kStride * 4; }
+// MATS = 2: gate and up, from x to h.  MATS = 1: down, from h to y.
+template <typename T, int MATS, int RH, int NT, int STAGES, int WK, int GROUP, bool ZERO>
+struct ExpertShape {
+    using Source = std::conditional_t<MATS == 2, RowSource<T>, std::conditional_t<sizeof(T) == 4, RowSource<float>, SplitSource>>;
+    using Product = WarpProduct<MATS * RH, NT, STAGES, GROUP, ZERO, Source>;
+    static constexpr int kGroups = kMoeWarps / WK;      // row groups of a unit
+    static constexpr int kOut = MATS * RH * NT * 128;   // a warp's sums
+    static constexpr int kRings = kMoeWarps * Product::kWarpBytes, kSmem = kRings + kMoeWarps * kOut * 4;
 };
 
-template <typename T, int R, int NT, int STAGES, int GROUP, bool ZERO>
-__global__ void __launch_bounds__(kMoeThreads) moe_down_kernel(const ExpertParams p) {
-    using Shape = DownShape<T, R, NT, STAGES, GROUP, ZERO>;
-    extern __shared__ __align__(16) uint8_t smem[];
-    float* sums = reinterpret_cast<float*>(smem + Shape::kRings);  // [warp][token][kStride]
+template <typename T, int MATS, int RH, int NT, int STAGES, int WK, int GROUP, bool ZERO>
+__global__ void __launch_bounds__(kMoeThreads) moe_expert_kernel(const ExpertParams p) {
+    using Shape = ExpertShape<T, MATS, RH, NT, STAGES, WK, GROUP, ZERO>;
+    constexpr int kOut = Shape::kOut;
+    extern __shared__ __align__(16) uint8_t smem[];  // the warps' rings, then their sums
     __shared__ PairLists lists;
-    cg::cluster_group cluster = cg::this_cluster();
-    const int split = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
-    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-    const int block0 = static_cast<int>(blockIdx.x) / split * R;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, group = warp / WK, part = warp % WK;
+    const Weight& first = MATS == 2 ? p.gate : p.down;
+    // The next kernels look at ids (and weights) before they wait for this one.  They start when every CTA of the product
+    // with gate and up has come to its trigger, which is after its wait: whatever made ids is complete by then.
+    if (MATS == 2) pdl_wait();
     pdl_trigger();
-    pdl_wait();
-    const int per_warp = p.T * Shape::kStride;
-    for (int i = threadIdx.x; i < kMoeWarps * per_warp; i += kMoeThreads) sums[i] = 0.0f;
     build_lists(lists, p.ids, p.T, p.top_k, p.E, 8 * NT);
-
-    float* mine = sums + warp * per_warp;
-    const int row_steps = ceil_div(p.down.k_blocks, 2), parts = split * kMoeWarps, part = rank * kMoeWarps + warp;
-    const long long steps = static_cast<long long>(lists.n_segments) * row_steps;
-    long long step = steps * part / parts;
-    const long long end = steps * (part + 1) / parts;
-    while (step < end) {
-        const int seg = static_cast<int>(step / row_steps), s0 = static_cast<int>(step - static_cast<long long>(seg) * row_steps);
-        const int s1 = static_cast<int>(min(static_cast<long long>(row_steps), s0 + (end - step)));
-        step += s1 - s0;
+    if (MATS == 1) pdl_wait();
+    const int row_blocks = first.row_blocks, chunks = ceil_div(row_blocks, RH * Shape::kGroups), units = lists.n_segments * chunks;
+    const int steps = ceil_div(first.k_blocks, 2), s0 = steps * part / WK, s1 = steps * (part + 1) / WK;
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+        const int seg = u / chunks, group0 = (u - seg * chunks) * Shape::kGroups, block0 = (group0 + group) * RH;
         const Segment sg = lists.segments[seg];
         typename Shape::Product product;
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-            product.set_rows(r, p.down, sg.expert, min(block0 + r, p.down.row_blocks - 1), lane);
+        for (int r = 0; r < RH; ++r) {
+            const int block = min(block0 + r, row_blocks - 1);
+            product.set_rows(r, first, sg.expert, block, lane);
+            if (MATS == 2) product.set_rows(RH + r, p.up, sg.expert, block, lane);
+        }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const int pair = lists.order[sg.first + min(8 * n + lane / 4, sg.columns - 1)], k = 8 * (lane & 3);
-            const size_t at = static_cast<size_t>(pair) * p.h_stride + k;
-            if constexpr (sizeof(T) == 4) product.x[n] = {static_cast<const float*>(p.h) + at, p.h_stride - k, true};
-            else product.x[n] = {static_cast<const __nv_bfloat16*>(p.h) + at, p.h_stride - k, p.h_low};
-        }
-        product.set_columns(p.h_stride);
-        float acc[R][NT][4] = {};
-        product.run(smem + warp * Shape::Product::kWarpBytes, s0, s1, lane, acc);
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int col = 8 * n + 2 * (lane & 3) + c;
-                if (col >= sg.columns) continue;
-                const int pair = lists.order[sg.first + col], token = pair / p.top_k;
-                float weight = 0.0f;
-                for (int j = pair; j < (token + 1) * p.top_k; ++j)
-                    if (j == pair || p.ids[j] == sg.expert) weight += p.weights[j];
-                // A segment's columns are distinct tokens: no two lanes add to the same sum.
-#pragma unroll
-                for (int r = 0; r < R; ++r)
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        float* at = mine + token * Shape::kStride + 16 * r + lane / 4 + 8 * half;
-                        *at = fmaf(weight, acc[r][n][2 * half + c], *at);
-                    }
+            if constexpr (MATS == 2) {
+                product.x[n] = {static_cast<const T*>(p.x) + static_cast<long long>(pair / p.top_k) * p.ldx + k, p.D - k, p.vec};
+            } else {
+                const size_t at = static_cast<size_t>(pair) * p.h_stride + k;
+                if constexpr (sizeof(T) == 4) product.x[n] = {static_cast<const float*>(p.h) + at, p.h_stride - k, true};
+                else product.x[n] = {static_cast<const __nv_bfloat16*>(p.h) + at, p.h_stride - k, p.h_low};
             }
-        __syncwarp();
+        }
+        product.set_columns(MATS == 2 ? (p.vec ? p.D : 0) : p.h_stride);
+        float acc[MATS * RH][NT][4] = {};
+        if (block0 < row_blocks) product.run(smem + warp * Shape::Product::kWarpBytes, s0, s1, lane, acc);
+        float* partial = reinterpret_cast<float*>(smem + Shape::kRings);
+#pragma unroll
+        for (int r = 0; r < MATS * RH; ++r)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) partial[warp * kOut + ((r * NT + n) * 4 + i) * 32 + lane] = acc[r][n][i];
+        __syncthreads();
+        constexpr int kEach = RH * NT * 128;
+        for (int i = threadIdx.x; i < Shape::kGroups * kEach; i += kMoeThreads) {
+            const int gr = i / kEach, j = i - gr * kEach;
+            const float* from = partial + gr * WK * kOut + j;
+            float a = 0.0f, b = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WK; ++w) {
+                a += from[w * kOut];
+                if (MATS == 2) b += from[w * kOut + kEach];
+            }
+            const int l = j & 31, f = (j >> 5) & 3, n = (j >> 7) % NT, r = (j >> 7) / NT;
+            const int row = ((group0 + gr) * RH + r) * 16 + l / 4 + 8 * (f >> 1), col = 8 * n + 2 * (l & 3) + (f & 1);
+            if (row >= row_blocks * 16 || col >= sg.columns) continue;
+            const size_t pair = static_cast<size_t>(lists.order[sg.first + col]);
+            if constexpr (MATS == 1) {
+                p.y[pair * p.y_stride + row] = a;
+            } else {
+                // Rows past F (up to the row block's end) are zeros, which the next product may read.
+                const float h = row < p.F ? a / (1.0f + expf(-a)) * b : 0.0f;
+                const size_t at = pair * p.h_stride + row;
+                if constexpr (sizeof(T) == 4) {
+                    static_cast<float*>(p.h)[at] = h;
+                } else {
+                    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.h) + at;
+                    dst[0] = __ushort_as_bfloat16(static_cast<unsigned short>(__float_as_uint(h) >> 16));
+                    dst[p.h_low] = __float2bfloat16_rn(after_bf16(h));
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// out[t] = sum over a token's counted pairs, in their order, of the weight times y.  4 elements a thread.
+constexpr int kCombineThreads = 128;
+
+template <typename T>
+__global__ void __launch_bounds__(kCombineThreads) moe_combine_kernel(const ExpertParams p) {
+    __shared__ float weight[kMaxTopK];  // 0: not counted
+    __shared__ bool counts[kMaxTopK];
+    const int t = blockIdx.y, d = (blockIdx.x * kCombineThreads + threadIdx.x) * 4;
+    pdl_trigger();
+    if (static_cast<int>(threadIdx.x) < p.top_k) {
+        const int j = threadIdx.x, id = counted_id(p.ids, t * p.top_k + j, p.top_k, p.E);
+        float w = 0.0f;
+        for (int q = j; q < p.top_k; ++q)
+            if (q == j || p.ids[t * p.top_k + q] == id) w += p.weights[t * p.top_k + q];
+        weight[j] = w;
+        counts[j] = id >= 0;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < per_warp; i += kMoeThreads) {
-        float v = sums[i];
+    pdl_wait();
+    if (d >= p.D) return;
+    float v[4] = {};
+    for (int j = 0; j < p.top_k; ++j) {
+        if (!counts[j]) continue;
+        const float4 y = *reinterpret_cast<const float4*>(p.y + static_cast<size_t>(t * p.top_k + j) * p.y_stride + d);
+        v[0] = fmaf(weight[j], y.x, v[0]);
+        v[1] = fmaf(weight[j], y.y, v[1]);
+        v[2] = fmaf(weight[j], y.z, v[2]);
+        v[3] = fmaf(weight[j], y.w, v[3]);
+    }
+    T* to = static_cast<T*>(p.out) + static_cast<size_t>(t) * p.D + d;
 #pragma unroll
-        for (int w = 1; w < kMoeWarps; ++w) v += sums[w * per_warp + i];
-        sums[i] = v;
+    for (int i = 0; i < 4; ++i) {
+        if (d + i >= p.D) break;
+        if constexpr (sizeof(T) == 4) to[i] = v[i];
+        else to[i] = __float2bfloat16_rn(v[i]);
     }
-    cluster.sync();
-    const int outputs = p.T * Shape::kRows;
-    for (int i = rank * kMoeThreads + threadIdx.x; i < outputs; i += split * kMoeThreads) {
-        const int token = i / Shape::kRows, r = i - token * Shape::kRows, row = block0 * 16 + r;
-        float v = 0.0f;
-        for (int s = 0; s < split; ++s) v += cluster.map_shared_rank(sums, s)[token * Shape::kStride + r];
-        if (row < p.D) {
-            T* dst = static_cast<T*>(p.out) + static_cast<size_t>(token) * p.D + row;
-            if constexpr (sizeof(T) == 4) *dst = v;
-            else *dst = __float2bfloat16_rn(v);
-        }
-    }
-    cluster.sync();  // no CTA leaves while another reads its sums
 }
 
 // ---- host -----------------------------------------------------------------------------------
@@ -549,45 +544,45 @@ inline int tokens_per_launch(int top_k) {
     return t < kMaxTokens ? t : kMaxTokens;
 }
 
-template <typename T, int RH, int NT, int STAGES, int GROUP, bool ZERO>
-int launch_gate_up(const ExpertParams& p, int sms, int dev, cudaStream_t stream) {
-    using Shape = GateUpShape<T, RH, NT, STAGES, GROUP, ZERO>;
-    constexpr auto kernel = moe_gate_up_kernel<T, RH, NT, STAGES, GROUP, ZERO>;
+template <typename T, int MATS, int RH, int NT, int STAGES, int WK, int GROUP, bool ZERO>
+int launch_experts(const ExpertParams& p, int sms, int dev, cudaStream_t stream) {
+    using Shape = ExpertShape<T, MATS, RH, NT, STAGES, WK, GROUP, ZERO>;
+    constexpr auto kernel = moe_expert_kernel<T, MATS, RH, NT, STAGES, WK, GROUP, ZERO>;
+    static_assert(Shape::kSmem <= 200 * 1024, "shared memory of a CTA");
     const int per_sm = resident_ctas<kernel>(dev, kMoeThreads, Shape::kSmem);
     if (per_sm < 1) return HGEMM_ERR_CUDA;
     const int pairs = p.T * p.top_k, experts = pairs < p.E ? pairs : p.E;
-    const long long most = static_cast<long long>(experts + pairs / (8 * NT)) * ceil_div(p.gate.row_blocks, RH);
+    const Weight& w = MATS == 2 ? p.gate : p.down;
+    const long long most = static_cast<long long>(experts + pairs / (8 * NT)) * ceil_div(w.row_blocks, RH * Shape::kGroups);
     const long long wave = static_cast<long long>(sms) * per_sm;
     return launch<kernel>(dim3(static_cast<unsigned>(most < wave ? most : wave)), kMoeThreads, 1, Shape::kSmem, stream, p);
 }
 
-template <typename T, int R, int NT, int STAGES, int GROUP, bool ZERO>
-int launch_down(const ExpertParams& p, int sms, int dev, cudaStream_t stream) {
-    using Shape = DownShape<T, R, NT, STAGES, GROUP, ZERO>;
-    constexpr auto kernel = moe_down_kernel<T, R, NT, STAGES, GROUP, ZERO>;
-    if (resident_ctas<kernel>(dev, kMoeThreads, Shape::smem(kMaxTokens)) < 1) return HGEMM_ERR_CUDA;
-    const int groups = ceil_div(p.down.row_blocks, R);
-    int split = 1;
-    while (split < 8 && groups * split < 2 * sms) split *= 2;
-    return launch<kernel>(dim3(static_cast<unsigned>(groups) * split), kMoeThreads, split, Shape::smem(p.T), stream, p);
+// WK: 2 where that gives units enough, else 4.  Measured (bf16, groups of 128; WK = 2, 4, 8): 32 tokens through 6 of 64
+// experts of 4096 x 2048, gate and up 145, 148, 156 us, down 92, 102, 110; 4 tokens through 8 of 64 of
+// 2048 x 1024, 19.0, 20.9, 21.9 and 14.5, 12.5, 13.4; one token 10.2, 10.5, 9.6 and 7.3, 5.3, 5.4.  Two row
+// blocks of down (4 of gate and up) a warp: 120 us with one for down, but 177 instead of 145 for gate and
+// up, whose CTAs then fit an SM once instead of three times.
+template <typename T, int MATS, int NT, int GROUP, bool ZERO>
+int run_experts(const ExpertParams& p, int sms, int dev, cudaStream_t stream) {
+    constexpr int RH = MATS == 2 ? 1 : 2;
+    const int pairs = p.T * p.top_k, experts = pairs < p.E ? pairs : p.E;
+    const int units = experts * ceil_div((MATS == 2 ? p.gate : p.down).row_blocks, RH * 4);
+    if (units >= (MATS == 2 ? 2 : 4) * sms) return launch_experts<T, MATS, RH, NT, 3, 2, GROUP, ZERO>(p, sms, dev, stream);
+    return launch_experts<T, MATS, RH, NT, 3, 4, GROUP, ZERO>(p, sms, dev, stream);
 }
 
-template <typename T, int GROUP, bool ZERO>
-int run_gate_up(const ExpertParams& p, int sms, int dev, cudaStream_t stream) {
-    if constexpr (sizeof(T) == 4) {
-        return launch_gate_up<T, 1, 1, 4, GROUP, ZERO>(p, sms, dev, stream);
-    } else {
-        if (p.T * p.top_k <= 8 * p.E) return launch_gate_up<T, 1, 1, 4, GROUP, ZERO>(p, sms, dev, stream);
-        return launch_gate_up<T, 1, 2, 4, GROUP, ZERO>(p, sms, dev, stream);
+// Columns of a segment: 8, or 16 where an expert has more than 8 tokens on average (bf16 only: fp32's three terms
+// and two tiles of columns do not fit the registers).
+template <typename T, int MATS, int GROUP, bool ZERO>
+int run_expert_product(const ExpertParams& p, int sms, int dev, cudaStream_t stream) {
+    if constexpr (sizeof(T) == 2) {
+        if (p.T * p.top_k > 8 * p.E) return run_experts<T, MATS, 2, GROUP, ZERO>(p, sms, dev, stream);
     }
+    return run_experts<T, MATS, 1, GROUP, ZERO>(p, sms, dev, stream);
 }
 
-template <typename T, int GROUP, bool ZERO>
-int run_down(const ExpertParams& p, int sms, int dev, cudaStream_t stream) {
-    return launch_down<T, 2, 1, 3, GROUP, ZERO>(p, sms, dev, stream);
-}
-
-inline size_t h_stride(int F) { return static_cast<size_t>(ceil_div(F, kTileRows)) * kTileRows; }
+inline size_t padded_rows(int n) { return static_cast<size_t>(ceil_div(n, kTileRows)) * kTileRows; }
 
 }  // namespace hgw
 
@@ -612,10 +607,10 @@ int hgemm_moe_route(const void* x, int x_dtype, long long ldx, const void* route
     return x_dtype == HGEMM_DTYPE_F32 ? hgw::run_route<float>(p, s) : hgw::run_route<__nv_bfloat16>(p, s);
 }
 
-size_t hgemm_w4_moe_workspace_bytes(int T, int top_k, int F) {
-    if (T <= 0 || top_k <= 0 || top_k > hgw::kMaxTopK || F <= 0) return 0;
+size_t hgemm_w4_moe_workspace_bytes(int T, int top_k, int D, int F) {
+    if (T <= 0 || top_k <= 0 || top_k > hgw::kMaxTopK || D <= 0 || F <= 0) return 0;
     const int most = hgw::tokens_per_launch(top_k), tokens = T < most ? T : most;
-    return static_cast<size_t>(tokens) * top_k * hgw::h_stride(F) * 4;  // h: fp32, or two bf16
+    return static_cast<size_t>(tokens) * top_k * (hgw::padded_rows(F) + hgw::padded_rows(D)) * 4;  // h and y
 }
 
 int hgemm_w4_moe(const void* x, int x_dtype, long long ldx, const int* ids, const float* weights, int T, int top_k, int E,
@@ -644,7 +639,7 @@ int hgemm_w4_moe(const void* x, int x_dtype, long long ldx, const int* ids, cons
         if (hgw::misaligned(w->q, 16) || hgw::misaligned(w->scales, 16) || hgw::misaligned(w->zeros, 16))
             return HGEMM_ERR_ALIGNMENT;
     }
-    if (!workspace || workspace_bytes < hgemm_w4_moe_workspace_bytes(T, top_k, F)) return HGEMM_ERR_INVALID_VALUE;
+    if (!workspace || workspace_bytes < hgemm_w4_moe_workspace_bytes(T, top_k, D, F)) return HGEMM_ERR_INVALID_VALUE;
     if (hgw::misaligned(workspace, 16)) return HGEMM_ERR_ALIGNMENT;
     if (int rc = hgw::current_device(&sms, &dev)) return rc;
 
@@ -659,9 +654,12 @@ int hgemm_w4_moe(const void* x, int x_dtype, long long ldx, const int* ids, cons
     p.up = hgw::make_weight(up->q, up->scales, up->zeros, F, D, up->group);
     p.down = hgw::make_weight(down->q, down->scales, down->zeros, D, F, down->group);
     p.vec = !hgw::misaligned(x, 16) && D % 8 == 0 && p.ldx % (16 / size) == 0;
+    const int held = (T < most ? T : most) * top_k;  // pairs of a launch
     p.h = workspace;
-    p.h_stride = static_cast<int>(hgw::h_stride(F));
-    p.h_low = static_cast<long long>(T < most ? T : most) * top_k * p.h_stride;
+    p.h_stride = static_cast<int>(hgw::padded_rows(F));
+    p.h_low = static_cast<long long>(held) * p.h_stride;
+    p.y = static_cast<float*>(workspace) + static_cast<size_t>(held) * p.h_stride;
+    p.y_stride = static_cast<int>(hgw::padded_rows(D));
     // Launches of up to kMaxTokens tokens; they share the workspace, in stream order.
     for (int t0 = 0; t0 < T; t0 += most) {
         p.T = T - t0 < most ? T - t0 : most;
@@ -672,16 +670,21 @@ int hgemm_w4_moe(const void* x, int x_dtype, long long ldx, const int* ids, cons
         int rc = hgw::with_format(gate->group, gate->zeros != nullptr, [&](auto g, auto z) {
             constexpr int G = decltype(g)::value;
             constexpr bool Z = decltype(z)::value;
-            return x_dtype == HGEMM_DTYPE_F32 ? hgw::run_gate_up<float, G, Z>(p, sms, dev, s)
-                                              : hgw::run_gate_up<__nv_bfloat16, G, Z>(p, sms, dev, s);
+            return x_dtype == HGEMM_DTYPE_F32 ? hgw::run_expert_product<float, 2, G, Z>(p, sms, dev, s)
+                                              : hgw::run_expert_product<__nv_bfloat16, 2, G, Z>(p, sms, dev, s);
         });
         if (rc) return rc;
         rc = hgw::with_format(down->group, down->zeros != nullptr, [&](auto g, auto z) {
             constexpr int G = decltype(g)::value;
             constexpr bool Z = decltype(z)::value;
-            return x_dtype == HGEMM_DTYPE_F32 ? hgw::run_down<float, G, Z>(p, sms, dev, s)
-                                              : hgw::run_down<__nv_bfloat16, G, Z>(p, sms, dev, s);
+            return x_dtype == HGEMM_DTYPE_F32 ? hgw::run_expert_product<float, 1, G, Z>(p, sms, dev, s)
+                                              : hgw::run_expert_product<__nv_bfloat16, 1, G, Z>(p, sms, dev, s);
         });
+        if (rc) return rc;
+        const dim3 grid(static_cast<unsigned>(hgw::ceil_div(D, 4 * hgw::kCombineThreads)), static_cast<unsigned>(p.T), 1);
+        rc = x_dtype == HGEMM_DTYPE_F32
+                 ? hgw::launch<hgw::moe_combine_kernel<float>>(grid, hgw::kCombineThreads, 1, 0, s, p)
+                 : hgw::launch<hgw::moe_combine_kernel<__nv_bfloat16>>(grid, hgw::kCombineThreads, 1, 0, s, p);
         if (rc) return rc;
     }
     return HGEMM_OK;

@@ -251,11 +251,11 @@ def moe_route(x: torch.Tensor, router: torch.Tensor, top_k: int, *, renormalize:
 def w4_moe(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate: W4Weight, up: W4Weight, down: W4Weight,
            out: torch.Tensor | None = None, *, workspace: torch.Tensor | None = None,
            stream: torch.cuda.Stream | None = None) -> torch.Tensor:
-    """The experts of a mixture for a few tokens (hgemm_w4_moe), in two kernels:
+    """The experts of a mixture for a few tokens (hgemm_w4_moe), in three kernels:
     out[t] = sum_j weights[t,j] * down_e(silu(gate_e x[t]) * (up_e x[t])), e = ids[t,j].
     x (T, D) fp32 or bf16, ids (T, top_k) int32 and weights (T, top_k) float32 as moe_route gives
     them (ids outside [0, E) add nothing), gate and up (E, F, D), down (E, D, F).  workspace:
-    hgemm_w4_moe_workspace_bytes(T, top_k, F) bytes that no other running call uses, else
+    hgemm_w4_moe_workspace_bytes(T, top_k, D, F) bytes that no other running call uses, else
     allocated by torch."""
     ldx, dt, dev = _check_rows("x", x)
     t, d = x.shape
@@ -280,7 +280,7 @@ def w4_moe(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate: W4We
         elif out.shape != (t, d) or out.dtype != x.dtype or not out.is_contiguous() or out.get_device() != dev:
             raise ValueError("out must be a contiguous (T, D) tensor of x's type on x's device")
         if workspace is None:
-            workspace = x.new_empty(_fn("hgemm_w4_moe_workspace_bytes")(t, top_k, f), dtype=torch.uint8)
+            workspace = x.new_empty(_fn("hgemm_w4_moe_workspace_bytes")(t, top_k, d, f), dtype=torch.uint8)
         elif workspace.get_device() != dev or not workspace.is_contiguous():
             raise ValueError("workspace must be a contiguous tensor on x's device")
         # Three hgemm_w4_weight: q, scales, zeros, group.

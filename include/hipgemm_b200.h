@@ -328,13 +328,13 @@ typedef struct {
     int group;
 } hgemm_w4_weight;
 
-/* The experts of a few tokens, in two kernels:
+/* The experts of a few tokens, in three kernels:
  *   out[t] = sum_j weights[t][j] * down_e( silu(gate_e x[t]) * (up_e x[t]) ),  e = ids[t][j].
  * x: T x D fp32 or bf16, `ldx` elements from row to row; out: T x D row-major of the same type;
  * gate and up: stacks of E (F x D) of the same group size, both with or both without zero
  * points; down: a stack of E (D x F).  An id outside [0, E) adds nothing (padding, experts of
  * another rank); an id that a token has twice counts with both weights.  Sums in fp32; the
- * product between the two kernels is kept in 16 significant bits or more.  Codes of an expert are
+ * product between the matrices is kept in 16 significant bits or more.  Codes of an expert are
  * read once per 8 or 16 of its tokens; tokens beyond 64 (or 512 / top_k) take further launches.  The
  * result's bits depend on the inputs alone.
  * workspace: device memory, 16-byte aligned, hgemm_w4_moe_workspace_bytes(); its content does not
@@ -343,7 +343,7 @@ typedef struct {
 int hgemm_w4_moe(const void* x, int x_dtype, long long ldx, const int* ids, const float* weights, int T, int top_k, int E,
                  int D, int F, const hgemm_w4_weight* gate, const hgemm_w4_weight* up, const hgemm_w4_weight* down,
                  void* out, void* workspace, size_t workspace_bytes, hgemm_stream_t stream);
-size_t hgemm_w4_moe_workspace_bytes(int T, int top_k, int F);
+size_t hgemm_w4_moe_workspace_bytes(int T, int top_k, int D, int F);
 
 /* ---- host utilities mirroring the reference harness (utils.hpp) ---------------------- */
 

@@ -173,7 +173,7 @@ def test_experts_strides_guards_and_workspace(cuda_device, dtype):
         rows = buf[at:at + t * (d + pad)].view(t, d + pad)[:, :d]
         rows.copy_(x)
         out = torch.full((t + 2, d), -3.0, dtype=dtype).cuda()
-        need = hg.lib().hgemm_w4_moe_workspace_bytes(t, top_k, f)
+        need = hg.lib().hgemm_w4_moe_workspace_bytes(t, top_k, d, f)
         ws = torch.full((need + 64,), 0xFF, dtype=torch.uint8).cuda()  # NaN patterns
         got = hg.w4_moe(rows, ids.cuda(), weights.cuda(), *packed, out=out[1:-1], workspace=ws[:need])
         ref.assert_close(got, *ref.experts(x, ids, weights, *dense, TERMS[dtype]), dtype)

@@ -20,11 +20,12 @@ def test_buffer_sizes():
     assert L.hgemm_w4_q_bytes(0, 8) == L.hgemm_w4_q_bytes(8, 0) == L.hgemm_w4_scales(8, 8, 16) == 0
     # Sizes beyond 32 bits.
     assert L.hgemm_w4_q_bytes(1 << 20, 1 << 20) == 1 << 39
-    assert L.hgemm_w4_moe_workspace_bytes(1, 8, 1000) == 8 * 1008 * 4
+    assert L.hgemm_w4_moe_workspace_bytes(1, 8, 33, 1000) == 8 * (48 + 1008) * 4
     # At most 64 tokens or 512 pairs are held at a time.
-    assert L.hgemm_w4_moe_workspace_bytes(1000, 8, 16) == 512 * 16 * 4
-    assert L.hgemm_w4_moe_workspace_bytes(1000, 3, 16) == 64 * 3 * 16 * 4
-    assert L.hgemm_w4_moe_workspace_bytes(0, 8, 16) == L.hgemm_w4_moe_workspace_bytes(4, 17, 16) == 0
+    assert L.hgemm_w4_moe_workspace_bytes(1000, 8, 32, 16) == 512 * 48 * 4
+    assert L.hgemm_w4_moe_workspace_bytes(1000, 3, 32, 16) == 64 * 3 * 48 * 4
+    assert L.hgemm_w4_moe_workspace_bytes(0, 8, 32, 16) == L.hgemm_w4_moe_workspace_bytes(4, 17, 32, 16) == 0
+    assert L.hgemm_w4_moe_workspace_bytes(4, 2, 0, 16) == L.hgemm_w4_moe_workspace_bytes(4, 2, 16, 0) == 0
 
 
 @pytest.mark.parametrize("lead,n,k,group", [((), 1, 1, 32), ((), 16, 64, 64), ((), 37, 130, 128), ((3,), 20, 97, 32)])
