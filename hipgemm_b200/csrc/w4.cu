@@ -542,16 +542,18 @@ int launch_linear(const LinearParams& p, int sms, int dev, cudaStream_t stream) 
 // and codes are all that streams.  After every kBatch row blocks the warps' sums are added up in
 // shared memory, then the CTAs' in distributed shared memory, in a fixed order.
 
-template <typename T, int MT, int XS, int GROUP, bool ZERO, int WARPS>
+constexpr int kRowsWarps = 16;
+
+template <typename T, int MT, int XS, int GROUP, bool ZERO>
 struct RowsShape {
-    // 10 KB of codes and scales a warp of 16 (20 KB of 8) are in flight or in use: 160 KB an SM.
+    // 10 KB of codes and scales a warp are in flight or in use: 160 KB an SM.
     static constexpr int kOneStage = WarpStationary<T, MT, XS, 1, GROUP, ZERO>::kStageBytes;
-    static constexpr int kStages = (WARPS == 16 ? 10240 : 20480) / kOneStage;
+    static constexpr int kStages = 10240 / kOneStage;
     static_assert(kStages >= 2, "a stage ahead");
     using Product = WarpStationary<T, MT, XS, kStages, GROUP, ZERO>;
     static constexpr int kBatch = MT == 0 ? 8 : 2;
-    static constexpr int kRings = WARPS * Product::kWarpBytes;
-    static constexpr int kBatchFloats = kBatch * WARPS * Product::kResult;  // [row block][warp][kResult]
+    static constexpr int kRings = kRowsWarps * Product::kWarpBytes;
+    static constexpr int kBatchFloats = kBatch * kRowsWarps * Product::kResult;  // [row block][warp][kResult]
     static constexpr int kExchange = kBatch * 16 * Product::kColumns;       // a CTA's sums: [column][row block][row]
     static constexpr int kSmem = kRings + 2 * (kBatchFloats + kExchange) * 4;
 };
@@ -559,11 +561,11 @@ struct RowsShape {
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-template <typename T, int MT, int XS, int GROUP, bool ZERO, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32, 1) w4_rows_kernel(const LinearParams p) {
-    using Shape = RowsShape<T, MT, XS, GROUP, ZERO, WARPS>;
+template <typename T, int MT, int XS, int GROUP, bool ZERO>
+__global__ void __launch_bounds__(kRowsWarps * 32, 1) w4_rows_kernel(const LinearParams p) {
+    using Shape = RowsShape<T, MT, XS, GROUP, ZERO>;
     using Product = typename Shape::Product;
-    constexpr int kStages = Shape::kStages, kBatch = Shape::kBatch, kThreads = WARPS * 32;
+    constexpr int kStages = Shape::kStages, kBatch = Shape::kBatch, kThreads = kRowsWarps * 32;
     extern __shared__ __align__(16) uint8_t smem[];
     float* partial = reinterpret_cast<float*>(smem + Shape::kRings);
     float* exchange = partial + 2 * Shape::kBatchFloats;
@@ -576,7 +578,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) w4_rows_kernel(const LinearPara
     const int end = static_cast<int>(static_cast<long long>(p.w.row_blocks) * (id + 1) / clusters);
 
     Product product;
-    product.set_slice(smem + warp * Product::kWarpBytes, (rank * WARPS + warp) * 2 * XS, p.w.k_blocks, lane);
+    product.set_slice(smem + warp * Product::kWarpBytes, (rank * kRowsWarps + warp) * 2 * XS, p.w.k_blocks, lane);
 #pragma unroll
     for (int m = 0; m < Product::kRowTiles; ++m) {
         // Columns past M repeat the last row; their sums are not stored.
@@ -622,7 +624,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) w4_rows_kernel(const LinearPara
             copy_commit();
             copy_wait<kStages - 1>();
             __syncwarp();
-            product.compute(stage, flip, high, sums + (i * WARPS + warp) * Product::kResult, lane);
+            product.compute(stage, flip, high, sums + (i * kRowsWarps + warp) * Product::kResult, lane);
             stage = stage == kStages - 1 ? 0 : stage + 1;
         }
         __syncthreads();
@@ -636,10 +638,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) w4_rows_kernel(const LinearPara
         float* out = exchange + buffer * Shape::kExchange;
         for (int i = threadIdx.x; i < columns * batch * 16; i += kThreads) {
             const int column = i / (batch * 16), r = i - column * (batch * 16);
-            const float* from = sums + r / 16 * (WARPS * Product::kResult) + column * Product::kSumStride + r % 16;
+            const float* from = sums + r / 16 * (kRowsWarps * Product::kResult) + column * Product::kSumStride + r % 16;
             float v = from[0];
 #pragma unroll
-            for (int w = 1; w < WARPS; ++w) v += from[w * Product::kResult];
+            for (int w = 1; w < kRowsWarps; ++w) v += from[w * Product::kResult];
             if (split == 1) finish(base, column, r, v);
             else out[i] = v;
         }
@@ -668,8 +670,8 @@ int resident_clusters(int split, int sms, int dev) {
     std::atomic<int>& slot = known[dev][split / 2];
     int n = slot.load(std::memory_order_relaxed);
     if (n == 0) {
-        constexpr auto kernel = w4_rows_kernel<__nv_bfloat16, 0, 1, 128, false, 16>;
-        constexpr int smem = RowsShape<__nv_bfloat16, 0, 1, 128, false, 16>::kSmem;
+        constexpr auto kernel = w4_rows_kernel<__nv_bfloat16, 0, 1, 128, false>;
+        constexpr int smem = RowsShape<__nv_bfloat16, 0, 1, 128, false>::kSmem;
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3(static_cast<unsigned>(sms / split * split), 1, 1);
         cfg.blockDim = dim3(512, 1, 1);
@@ -690,8 +692,9 @@ int resident_clusters(int split, int sms, int dev) {
     return n;
 }
 
-// Candidate `split`, for warps that may hold up to `most` steps.  The cost is a warp's steps from begin to end, and
-// two for the exchange between CTAs.
+// Candidate `split`, for warps that may hold up to `most` steps.  The cost is a warp's steps from begin to end, two
+// for each step of x that it turns into planes, and one for the exchange between CTAs (8192 x 8192 by one row: 13.5
+// us for 1 CTA, 11.4 for 2 and 12.7 for 4; 28672 x 8192: 27.0, 25.6, 33).
 inline RowsPlan rows_plan(int row_blocks, int steps, int split, int clusters, int warps, int most) {
     RowsPlan plan;
     int held = ceil_div(steps, split * warps);
@@ -700,18 +703,18 @@ inline RowsPlan rows_plan(int row_blocks, int steps, int split, int clusters, in
     plan.split = split;
     plan.steps = held;
     plan.clusters = clusters < row_blocks ? clusters : row_blocks;
-    plan.cost = static_cast<long long>(ceil_div(row_blocks, plan.clusters)) * held + (split > 1 ? 2 : 0);
+    plan.cost = static_cast<long long>(ceil_div(row_blocks, plan.clusters) + 2) * held + (split > 1 ? 1 : 0);
     return plan;
 }
 
-template <typename T, int MT, int XS, int GROUP, bool ZERO, int WARPS>
+template <typename T, int MT, int XS, int GROUP, bool ZERO>
 int launch_rows(const LinearParams& p, const RowsPlan& plan, int dev, cudaStream_t stream) {
-    using Shape = RowsShape<T, MT, XS, GROUP, ZERO, WARPS>;
-    constexpr auto kernel = w4_rows_kernel<T, MT, XS, GROUP, ZERO, WARPS>;
+    using Shape = RowsShape<T, MT, XS, GROUP, ZERO>;
+    constexpr auto kernel = w4_rows_kernel<T, MT, XS, GROUP, ZERO>;
     static_assert(Shape::kSmem <= 227 * 1024, "shared memory of a CTA");
-    if (resident_ctas<kernel>(dev, WARPS * 32, Shape::kSmem) < 1) return HGEMM_ERR_CUDA;
+    if (resident_ctas<kernel>(dev, kRowsWarps * 32, Shape::kSmem) < 1) return HGEMM_ERR_CUDA;
     const unsigned columns = static_cast<unsigned>(ceil_div(p.M, Shape::Product::kColumns));
-    return launch<kernel>(dim3(static_cast<unsigned>(plan.clusters * plan.split), columns, 1), WARPS * 32, plan.split,
+    return launch<kernel>(dim3(static_cast<unsigned>(plan.clusters * plan.split), columns, 1), kRowsWarps * 32, plan.split,
                           Shape::kSmem, stream, p);
 }
 
@@ -719,23 +722,24 @@ int launch_rows(const LinearParams& p, const RowsPlan& plan, int dev, cudaStream
 template <typename T, int MT>
 struct RowsLimits {
     static constexpr int kTiles = MT == 0 ? 1 : MT * (sizeof(T) == 4 ? 4 : 3);
-    static constexpr int kWarps = kTiles <= 4 ? 16 : 8;
+    static_assert(kTiles <= 4, "16 warps leave 128 registers a thread");
     static constexpr int kSteps = kTiles == 1 ? 4 : 2;
 };
 
+// False where the plan costs less than `least` (too little work to hold x for) or K is too long for the warps' registers.
 template <typename T, int MT, int GROUP, bool ZERO>
-bool run_rows(const LinearParams& p, int sms, int dev, cudaStream_t stream, int* rc) {
+bool run_rows(const LinearParams& p, int least, int sms, int dev, cudaStream_t stream, int* rc) {
     using Limits = RowsLimits<T, MT>;
     RowsPlan best;
     for (int split = 1; split <= 4; split *= 2) {
         const RowsPlan plan = rows_plan(p.w.row_blocks, ceil_div(p.w.k_blocks, 2), split, resident_clusters(split, sms, dev),
-                                        Limits::kWarps, Limits::kSteps);
+                                        kRowsWarps, Limits::kSteps);
         if (plan.split && (!best.split || plan.cost < best.cost)) best = plan;
     }
-    if (!best.split) return false;  // K is too long for the warps' registers
-    if (best.steps == 1) *rc = launch_rows<T, MT, 1, GROUP, ZERO, Limits::kWarps>(p, best, dev, stream);
-    else if (best.steps == 2) *rc = launch_rows<T, MT, 2, GROUP, ZERO, Limits::kWarps>(p, best, dev, stream);
-    else if constexpr (Limits::kSteps >= 4) *rc = launch_rows<T, MT, 4, GROUP, ZERO, Limits::kWarps>(p, best, dev, stream);
+    if (!best.split || best.cost < least) return false;
+    if (best.steps == 1) *rc = launch_rows<T, MT, 1, GROUP, ZERO>(p, best, dev, stream);
+    else if (best.steps == 2) *rc = launch_rows<T, MT, 2, GROUP, ZERO>(p, best, dev, stream);
+    else if constexpr (Limits::kSteps >= 4) *rc = launch_rows<T, MT, 4, GROUP, ZERO>(p, best, dev, stream);
     return true;
 }
 
@@ -746,10 +750,18 @@ int run_tc(const void* x, long long ldx, void* y, int M, int N, int K, const Wei
 template <typename T, int GROUP, bool ZERO>
 int run_linear(const LinearParams& p, int sms, int dev, cudaStream_t stream) {
     int rc = 0;
-    if (p.M <= 2 && run_rows<T, 0, GROUP, ZERO>(p, sms, dev, stream, &rc)) return rc;
     if constexpr (sizeof(T) == 4) {
+        // Three matrix instructions for the three terms of x, and making the terms: x held in registers is faster nearly
+        // throughout (us here and there: 8192 x 8192 by 1 row 14.5 and 30.7, by 3 rows 19.4 and 31.2, by 16 39 and
+        // 57; 4096 x 1024 by 3 4.7 and 6.7), but for the least work (1024 x 1024 by 1: 3.6 and 3.1).
+        if (p.M <= 2 ? run_rows<T, 0, GROUP, ZERO>(p, 4, sms, dev, stream, &rc) : run_rows<T, 1, GROUP, ZERO>(p, 4, sms, dev, stream, &rc))
+            return rc;
         return launch_linear<T, 2, 1, 3, GROUP, ZERO, 4>(p, sms, dev, stream);
     } else {
+        // One or two rows: x held in registers pays where there is work enough (us here and there: 28672 x 8192 25.6 and
+        // 34.3, 7168 x 2048 4.8 and 5.6, 4096 x 1024 3.9 and 2.8).  Three to eight rows take three times the integer
+        // instructions: 8192 x 8192 16.5 and 12.7.
+        if (p.M <= 2 && run_rows<T, 0, GROUP, ZERO>(p, 6, sms, dev, stream, &rc)) return rc;
         // Measured at 8192 x 8192 (28672 x 8192): 16 rows 14.8 (46.4) us here and 14.5 (43.2) there, but 5.6 and 7.4 at 4096 x 4096;
         // 17 rows 28.5 (86.4) and 16.7 (51.7); 64 rows 44.3 (153) and 21.7 (68.2).
         if (p.M > 16 && p.vec) return run_tc(p.x, p.ldx, p.y, p.M, p.N, p.K, p.w, GROUP, sms, dev, stream);
