@@ -273,3 +273,120 @@ def test_wrapper_refusals(cuda_device):
         hg.quantize_w4(torch.zeros(4, 64).cuda(), group=100)
     with pytest.raises(TypeError):
         hg.quantize_w4(torch.zeros(4, 64, dtype=torch.float16).cuda())
+
+
+# ---- the kernels that small matrices do not reach --------------------------------------------------
+#
+# One or two rows, and any fp32 rows, of matrices large enough hold x in registers as whole numbers;
+# more than 16 bf16 rows go through the 5th-generation tensor cores.
+
+
+def _planes_off(x, values):
+    """What holding x as whole numbers may lose: half of the last place, 2^-21 of a power of two that is at most
+    twice the largest of the row (bf16; fp32 2^-28), for every element."""
+    last = 2.0 ** -21 if x.dtype == torch.bfloat16 else 2.0 ** -28
+    return last * x.double().abs().amax(1, keepdim=True) * values.abs().sum(1)
+
+
+@pytest.mark.parametrize("m,dtype", [(1, torch.bfloat16), (2, torch.bfloat16), (1, torch.float32), (2, torch.float32),
+                                     (3, torch.float32), (8, torch.float32), (11, torch.float32)])
+@pytest.mark.parametrize("n,k,group,zero_point", [(5120, 1024, 128, False), (7100, 1100, 32, True), (2500, 4000, 64, True),
+                                                  (4096, 2113, 128, True), (300, 20000, 64, False)])
+def test_linear_rows_in_registers(cuda_device, m, n, k, group, zero_point, dtype):
+    gen = _gen(m, n, k, group, 3)
+    w, values = _weight(gen, (n, k), group, zero_point)
+    x = torch.randn(m, k, generator=gen).to(dtype)
+    y, off = ref.linear(x, values, TERMS[dtype])
+    got = hg.w4_gemm_tn(x.cuda(), w)
+    ref.assert_close(got, y, off + _planes_off(x, values), dtype)
+    assert torch.equal(hg.w4_gemm_tn(x.cuda(), w), got)
+
+
+@pytest.mark.parametrize("m,dtype", [(1, torch.bfloat16), (2, torch.bfloat16), (2, torch.float32), (5, torch.float32),
+                                     (24, torch.bfloat16), (40, torch.bfloat16)])
+def test_linear_special_values_in_large_matrices(cuda_device, m, dtype):
+    """Rows with infinities, NaN, the largest and the smallest numbers, and outliers, beside ordinary ones."""
+    n, k = 5120, 1024
+    gen = _gen(m, 77)
+    codes, scales, _ = ref.random_weight(gen, (n, k), 64, False)
+    codes[codes == 8] = 9  # no weight is 0: infinity times 0 would be NaN
+    w, values = hg.w4_pack(codes.cuda(), scales.cuda(), group=64), ref.values(codes, scales, None, 64)
+    kinds = [lambda r: r.__setitem__(5, float("inf")), lambda r: r.__setitem__(700, float("nan")),
+             lambda r: r.mul_(2.0 ** 118), lambda r: r.mul_(2.0 ** -100), lambda r: r.__setitem__(3, -float("inf")),
+             lambda r: r.__setitem__(9, 5000.0), lambda r: r.zero_(), lambda r: None]
+    for first in range(len(kinds)):
+        x = torch.randn(m, k, generator=gen)
+        for i in range(min(m, 2)):
+            kinds[(first + i) % len(kinds)](x[-1 - i])
+        x = x.to(dtype)
+        got = hg.w4_gemm_tn(x.cuda(), w).cpu()
+        clean = torch.where(x.isfinite(), x, 0)
+        y, off = ref.linear(clean, values, TERMS[dtype])
+        for i in range(m):
+            bad = x[i][~x[i].isfinite()]
+            if bad.numel() == 0:
+                ref.assert_close(got[i:i + 1], y[i:i + 1], (off + _planes_off(clean, values))[i:i + 1], dtype)
+            elif bool(bad.isnan().any()):
+                assert bool(got[i].isnan().all())
+            else:
+                want = x[i].double()[~x[i].isfinite()] * values[:, ~x[i].isfinite()]  # one infinity
+                assert torch.equal(got[i].double(), want[:, 0])
+
+
+@pytest.mark.parametrize("m", [17, 32, 33, 63, 64, 65, 130])
+@pytest.mark.parametrize("n,k", [(128, 64), (1, 8), (100, 1000), (1000, 136), (513, 4104)])
+@pytest.mark.parametrize("group,zero_point", [(32, True), (64, False), (128, True)])
+def test_linear_many_rows(cuda_device, m, n, k, group, zero_point):
+    gen = _gen(m, n, k, group, 9)
+    w, values = _weight(gen, (n, k), group, zero_point)
+    x = torch.randn(m, k, generator=gen).bfloat16()
+    ref.assert_close(hg.w4_gemm_tn(x.cuda(), w), *ref.linear(x, values, 1), torch.bfloat16)
+    assert hg.device_status() == 0
+
+
+def test_linear_many_rows_strides_guards_and_graphs(cuda_device):
+    """Rows that are strided (aligned, so that the tensor-core kernel takes them, and not), NaN between and behind
+    them, rows of the output behind the last, a captured graph, another stream, and two streams at once."""
+    gen = _gen(31)
+    n, k = 700, 520
+    w, values = _weight(gen, (n, k), 32, True)
+    for m, pad, at in [(20, 8, 0), (40, 24, 8), (33, 3, 1), (70, 0, 0)]:
+        x = torch.randn(m, k, generator=gen).bfloat16()
+        buf = torch.full((at + (m + 1) * (k + pad),), float("nan"), dtype=torch.bfloat16).cuda()
+        rows = buf[at:at + m * (k + pad)].view(m, k + pad)[:, :k]
+        rows.copy_(x)
+        out = torch.full((m + 2, n), -3.0, dtype=torch.bfloat16).cuda()
+        first = hg.w4_gemm_tn(rows, w, out=out[1:-1]).clone()
+        ref.assert_close(first, *ref.linear(x, values, 1), torch.bfloat16)
+        assert bool((out[0] == -3).all()) and bool((out[-1] == -3).all())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            hg.w4_gemm_tn(rows, w, out=out[1:-1])
+        for _ in range(3):
+            out[1:-1].fill_(float("nan"))
+            graph.replay()
+            assert torch.equal(out[1:-1], first)
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+        got = [[hg.w4_gemm_tn(rows, w, stream=s) for s in streams] for _ in range(8)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, first) for pair in got for g in pair)
+    assert hg.device_status() == 0
+
+
+def test_a_call_for_each_kernel_in_a_row(cuda_device):
+    """Products of 1, 2, 5, 16 and 48 rows one after the other on one stream, each on the one before's output."""
+    gen = _gen(41)
+    size = 2048
+    w, values = _weight(gen, (size, size), 128, False)
+    x = torch.randn(48, size, generator=gen).bfloat16().cuda()
+    outs = []
+    for m in (48, 16, 5, 2, 1):
+        x = hg.w4_gemm_tn(x[:m], w)
+        outs.append(x)
+    torch.cuda.synchronize()
+    for before, got in zip(outs, outs[1:]):
+        y = before[:got.shape[0]].cpu()
+        want, off = ref.linear(y, values, 1)
+        ref.assert_close(got, want, off + _planes_off(y, values), torch.bfloat16)
