@@ -32,8 +32,10 @@ constexpr int kMaxSegments = kMaxPairs;
 // experts, EW at a time, so that a load of x serves EW experts and one of the router TT tokens.
 // Sixteen products a lane are summed in fp32 and then added in 64 bits, so that experts whose logits
 // are close are ordered as the exact logits are.  The logits go to the CTA that selects the
-// token's experts over distributed shared memory.  Bound by the latency of the router's loads
-// (each cluster reads all of it from L2): hence 16 warps, and two loads of each row at a time.
+// token's experts over distributed shared memory.  Bound by the latency of the router's loads, all of
+// which each cluster reads from L2: hence two loads of each row at a time, in a branch without other
+// conditions (64 tokens, 7168 x 256 fp32: 32.5 us, 48 with a condition a load), and two CTAs an SM.
+// One token, 2048 x 128 bf16: 5.8 us.
 
 constexpr int kRouteCluster = 8;
 constexpr int kRouteWarps = 8;

@@ -170,6 +170,8 @@ __device__ __forceinline__ void encode8(const float (&w0)[8], const float (&w1)[
 // has rows g and g + 8, K 8 t .. 8 t + 7 of each 32: exactly the codes of its own 16 bytes, so
 // nothing is exchanged but the extremes (two shuffles over t) and the scales, of which lane t
 // works out those of group t.  HBM-bound in the main: w is read once; about 8 instructions an element.
+// 28672 x 8192 bf16 to codes and back takes 241 us, 4.9 TB/s of the two kernels' traffic (a division an
+// element made it 697); 4999 x 5115 fp32, whose rows go through shared memory, 72 us (scalar loads 211).
 template <typename T, bool ZERO, int GROUP, bool VEC>
 __global__ void __launch_bounds__(kQuantThreads) quantize_w4_kernel(const T* __restrict__ w, int N, int K, int row_blocks,
                                                                     int k_blocks, int groups, unsigned items,
@@ -430,6 +432,8 @@ int run_dequantize(const Weight& v, int count, int N, int K, T* w, int sms, int 
 // takes R row blocks; its warps split K, and a cluster of `split` CTAs splits it again where
 // there are too few row blocks for the GPU.  The partial sums are joined in a fixed order, over
 // shared memory and then distributed shared memory: the bits do not depend on timing.
+// Two row blocks a warp and 3 stages were the best of 1, 2 and 4 by 3 and 4 (28672 x 8192 by one
+// row: 34, against 36 with one block and 38 with four; by 16 rows 46, 58 and 58 us).
 
 struct LinearParams {
     const void* x;
@@ -539,7 +543,9 @@ int launch_linear(const LinearParams& p, int sms, int dev, cudaStream_t stream) 
 //
 // A persistent grid, one CTA an SM: a cluster of `split` CTAs takes a range of row blocks, its warps
 // a slice of K each for all of them, so that x is read and turned into whole numbers once per warp
-// and codes are all that streams.  After every kBatch row blocks the warps' sums are added up in
+// and codes are all that streams: 62 instructions a tile instead of 88.  28672 x 8192 by one row takes
+// 25.6 us (4.7 TB/s) instead of 34; what is left is start and end (4.8 us for 7168 x 2048, most of it
+// launch, the planes and the first bytes' latency).  After every kBatch row blocks the warps' sums are added up in
 // shared memory, then the CTAs' in distributed shared memory, in a fixed order.
 
 constexpr int kRowsWarps = 16;

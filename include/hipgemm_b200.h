@@ -305,9 +305,13 @@ int hgemm_dequantize_w4(const void* q, const void* scales, const void* zeros, in
 
 /* y[M x N] = x[M x K] . W[N x K]^T for few rows of x (decoding): x fp32 or bf16 with `ldx`
  * elements from row to row, y row-major of the same type, sums in fp32, one rounding.  x is used
- * as it is (fp32 in full).  Any M, N, K; y is fully overwritten; K == 0 writes zeros.  W is read
- * once per 8 rows of fp32 or 32 rows of bf16 x, so for many rows dequantise it instead.  The
- * result's bits depend on the inputs alone.  Needs no workspace.  x, y aligned to their element. */
+ * in full, except that for one or two rows, and for rows of fp32, it may be held in fixed point
+ * against the largest element of up to 512 consecutive K of its row: to half of 2^-21 (bf16) or
+ * 2^-28 (fp32) of that.  Any N and K, M <= 524280 (HGEMM_ERR_UNSUPPORTED above); y is fully
+ * overwritten; K == 0 writes zeros.  W is read once per 8 rows of fp32 or 16 to 64 of bf16 x, so
+ * for many rows dequantise it instead.  The result's bits depend on the inputs alone.  Needs no
+ * workspace.  x, y aligned to their element.  The first call on a device, outside any stream
+ * capture, as for the GEMM. */
 int hgemm_w4_gemm_tn(const void* x, int x_dtype, long long ldx, const void* q, const void* scales, const void* zeros,
                      void* y, int M, int N, int K, int group, hgemm_stream_t stream);
 
