@@ -414,7 +414,7 @@ struct SplitSource {
 template <typename T, int MATS, int RH, int NT, int STAGES, int WK, int GROUP, bool ZERO>
 struct ExpertShape {
     using Source = std::conditional_t<MATS == 2, RowSource<T>, std::conditional_t<sizeof(T) == 4, RowSource<float>, SplitSource>>;
-    using Product = WarpProduct<MATS * RH, NT, STAGES, GROUP, ZERO, Source>;
+    using Product = WarpProduct<MATS * RH, NT, STAGES, GROUP, ZERO, true, Source>;
     static constexpr int kGroups = kMoeWarps / WK;      // row groups of a unit
     static constexpr int kOut = MATS * RH * NT * 128;   // a warp's sums
     static constexpr int kRings = kMoeWarps * Product::kWarpBytes, kSmem = kRings + kMoeWarps * kOut * 4;

@@ -454,7 +454,7 @@ __device__ __forceinline__ void store<__nv_bfloat16>(__nv_bfloat16* p, float v) 
 // Shared memory: the warps' rings, and over them, once the products are done, their sums.
 template <typename T, int R, int NT, int STAGES, int GROUP, bool ZERO, int WARPS>
 struct LinearShape {
-    using Product = WarpProduct<R, NT, STAGES, GROUP, ZERO, RowSource<T>>;
+    using Product = WarpProduct<R, NT, STAGES, GROUP, ZERO, false, RowSource<T>>;
     static constexpr int kOut = R * NT * 128;  // a CTA's outputs: 16 R rows x 8 NT columns, in fragment order
     static constexpr int kRings = WARPS * Product::kWarpBytes, kSums = WARPS * kOut * 4;
     static constexpr int kSmem = kRings > kSums ? kRings : kSums;
