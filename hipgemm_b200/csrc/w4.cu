@@ -520,11 +520,12 @@ __global__ void __launch_bounds__(WARPS * 32) w4_linear_kernel(const LinearParam
     }
 }
 
-// CTAs of a cluster that share the K of a row group, for `groups` groups of rows: enough CTAs
-// for two on every SM, as long as a warp keeps two steps.
+// CTAs of a cluster that share the K of a row group, for `groups` groups of rows: enough CTAs for two on every SM, as
+// long as a warp keeps a step.  (With two steps at least, 8 rows of 4096 x 4096 took 7.0 us instead of 5.3, of
+// 1024 x 8192 6.3 instead of 4.8; 16 of 1024 x 1024 2.6 instead of 3.2.)
 inline int choose_split(int groups, int steps, int sms, int warps) {
     int split = 1;
-    while (split < 8 && groups * split < 2 * sms && steps >= 2 * split * warps * 2) split *= 2;
+    while (split < 8 && groups * split < 2 * sms && steps >= 2 * split * warps) split *= 2;
     return split;
 }
 
@@ -768,8 +769,9 @@ int run_linear(const LinearParams& p, int sms, int dev, cudaStream_t stream) {
         // 34.3, 7168 x 2048 4.8 and 5.6, 4096 x 1024 3.9 and 2.8).  Three to eight rows take three times the integer
         // instructions: 8192 x 8192 16.5 and 12.7.
         if (p.M <= 2 && run_rows<T, 0, GROUP, ZERO>(p, 6, sms, dev, stream, &rc)) return rc;
-        // Measured at 8192 x 8192 (28672 x 8192): 16 rows 14.8 (46.4) us here and 14.5 (43.2) there, but 5.6 and 7.4 at 4096 x 4096;
-        // 17 rows 28.5 (86.4) and 16.7 (51.7); 64 rows 44.3 (153) and 21.7 (68.2).
+        // The tensor cores from 17 rows on (us below and there, at 8192 x 8192 and at 28672 x 8192): 16 rows 14.8 and 14.5,
+        // 46.4 and 43.2, but 5.6 and 7.4 at 4096 x 4096; 17 rows 28.5 and 16.7, 86.4 and 51.7; 64 rows 44.3 and
+        // 21.7, 153 and 68.2.
         if (p.M > 16 && p.vec) return run_tc(p.x, p.ldx, p.y, p.M, p.N, p.K, p.w, GROUP, sms, dev, stream);
         if (p.M <= 8) return launch_linear<T, 2, 1, 3, GROUP, ZERO, 8>(p, sms, dev, stream);
         if (p.M <= 16) return launch_linear<T, 2, 2, 3, GROUP, ZERO, 4>(p, sms, dev, stream);
