@@ -199,7 +199,8 @@ struct RowSource<float> {
             }
         }
     }
-    // x = three bf16 by truncation, 8 significant bits each: 24 bits, so nothing is lost.
+    // x = three bf16 by truncation, 8 significant bits each: 24 bits, so nothing is lost (of |x| below 2^-110 what lies
+    // under bf16's smallest number, 2^-133).
     __device__ __forceinline__ static void terms(const Raw& raw, uint32_t (&b)[3][8]) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
