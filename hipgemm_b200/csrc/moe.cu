@@ -350,9 +350,10 @@ __device__ void build_lists(PairLists& s, const int* ids, int T, int top_k, int 
 // blocks (of gate and of up, or of down); WK warps split its K, and their sums are joined in shared
 // memory in a fixed order.
 //
-// h = silu(gate x) * (up x) is kept, for bf16 x, as two bf16 whose sum has 16 significant bits or more: twice
-// the matrix instructions in the product with down, and no rounding to 8 bits between the two
-// products, which would add as much error as the output's own rounding.  For fp32 x it is kept in fp32.
+// h = silu(gate x) * (up x) is kept in fp32 and enters the product with down as three bf16 terms, whose sum it
+// is: nothing between the two products is rounded to fewer bits.  As two bf16 (16 bits) it cost bf16 outputs
+// their last place more often than the order of summation does (2-norm of the difference to fp32's outputs
+// 1.3e-4 to 1.6e-4, now 2e-5 to 9e-5), and 240 us instead of 289 (32 tokens), 16.3 instead of 18.0 (one).
 
 struct ExpertParams {
     const void* x;
@@ -362,59 +363,18 @@ struct ExpertParams {
     int T, top_k, E, D, F;
     Weight gate, up, down;
     bool vec;
-    void* h;                // rows of h_stride elements by pair: fp32, or upper bf16 and h_low elements on the lower ones
+    float* h;               // rows of h_stride by pair
     int h_stride;           // F rounded up to whole row blocks
-    long long h_low;
     float* y;               // rows of y_stride by pair: down's products
     int y_stride;           // D rounded up to whole row blocks
     void* out;
 };
 
-// Rows of h as two bf16 terms, 16-byte aligned and a multiple of 16 long.
-struct SplitSource {
-    static constexpr int kTerms = 2;
-    struct Raw {
-        uint4 v[4];
-    };
-    const __nv_bfloat16* row;
-    int len;
-    long long low;
-    __device__ __forceinline__ void load_full(Raw& raw, int k) const {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            raw.v[h] = reinterpret_cast<const uint4*>(row + k)[4 * h];
-            raw.v[2 + h] = reinterpret_cast<const uint4*>(row + low + k)[4 * h];
-        }
-    }
-    __device__ __forceinline__ void load(Raw& raw, int k) const {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int at = k + 32 * h;
-            raw.v[h] = raw.v[2 + h] = make_uint4(0u, 0u, 0u, 0u);
-            if (at < len) {
-                raw.v[h] = *reinterpret_cast<const uint4*>(row + at);
-                raw.v[2 + h] = *reinterpret_cast<const uint4*>(row + low + at);
-            }
-        }
-    }
-    __device__ __forceinline__ static void terms(const Raw& raw, uint32_t (&b)[2][8]) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                b[s][4 * h] = raw.v[2 * s + h].x;
-                b[s][4 * h + 1] = raw.v[2 * s + h].y;
-                b[s][4 * h + 2] = raw.v[2 * s + h].z;
-                b[s][4 * h + 3] = raw.v[2 * s + h].w;
-            }
-    }
-};
-
 // MATS = 2: gate and up, from x to h.  MATS = 1: down, from h to y.
 template <typename T, int MATS, int RH, int NT, int STAGES, int WK, int GROUP, bool ZERO>
 struct ExpertShape {
-    using Source = std::conditional_t<MATS == 2, RowSource<T>, std::conditional_t<sizeof(T) == 4, RowSource<float>, SplitSource>>;
-    using Product = WarpProduct<MATS * RH, NT, STAGES, GROUP, ZERO, true, Source>;
+    using Source = std::conditional_t<MATS == 2, RowSource<T>, RowSource<float>>;
+    using Product = WarpProduct<MATS * RH, NT, STAGES, GROUP, ZERO, MATS == 2, Source>;
     static constexpr int kGroups = kMoeWarps / WK;      // row groups of a unit
     static constexpr int kOut = MATS * RH * NT * 128;   // a warp's sums
     static constexpr int kRings = kMoeWarps * Product::kWarpBytes, kSmem = kRings + kMoeWarps * kOut * 4;
@@ -452,9 +412,7 @@ __global__ void __launch_bounds__(kMoeThreads) moe_expert_kernel(const ExpertPar
             if constexpr (MATS == 2) {
                 product.x[n] = {static_cast<const T*>(p.x) + static_cast<long long>(pair / p.top_k) * p.ldx + k, p.D - k, p.vec};
             } else {
-                const size_t at = static_cast<size_t>(pair) * p.h_stride + k;
-                if constexpr (sizeof(T) == 4) product.x[n] = {static_cast<const float*>(p.h) + at, p.h_stride - k, true};
-                else product.x[n] = {static_cast<const __nv_bfloat16*>(p.h) + at, p.h_stride - k, p.h_low};
+                product.x[n] = {p.h + static_cast<size_t>(pair) * p.h_stride + k, p.h_stride - k, true};
             }
         }
         product.set_columns(MATS == 2 ? (p.vec ? p.D : 0) : p.h_stride);
@@ -486,15 +444,7 @@ __global__ void __launch_bounds__(kMoeThreads) moe_expert_kernel(const ExpertPar
                 p.y[pair * p.y_stride + row] = a;
             } else {
                 // Rows past F (up to the row block's end) are zeros, which the next product may read.
-                const float h = row < p.F ? a / (1.0f + expf(-a)) * b : 0.0f;
-                const size_t at = pair * p.h_stride + row;
-                if constexpr (sizeof(T) == 4) {
-                    static_cast<float*>(p.h)[at] = h;
-                } else {
-                    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.h) + at;
-                    dst[0] = __ushort_as_bfloat16(static_cast<unsigned short>(__float_as_uint(h) >> 16));
-                    dst[p.h_low] = __float2bfloat16_rn(after_bf16(h));
-                }
+                p.h[pair * p.h_stride + row] = row < p.F ? a / (1.0f + expf(-a)) * b : 0.0f;
             }
         }
         __syncthreads();
@@ -570,8 +520,9 @@ int run_experts(const ExpertParams& p, int sms, int dev, cudaStream_t stream) {
     constexpr int RH = MATS == 2 ? 1 : 2;
     const int pairs = p.T * p.top_k, experts = pairs < p.E ? pairs : p.E;
     const int units = experts * ceil_div((MATS == 2 ? p.gate : p.down).row_blocks, RH * 4);
-    if (units >= (MATS == 2 ? 2 : 4) * sms) return launch_experts<T, MATS, RH, NT, 3, 2, GROUP, ZERO>(p, sms, dev, stream);
-    return launch_experts<T, MATS, RH, NT, 3, 4, GROUP, ZERO>(p, sms, dev, stream);
+    using Of = std::conditional_t<MATS == 2, T, float>;  // down reads h, fp32 for either type of x
+    if (units >= (MATS == 2 ? 2 : 4) * sms) return launch_experts<Of, MATS, RH, NT, 3, 2, GROUP, ZERO>(p, sms, dev, stream);
+    return launch_experts<Of, MATS, RH, NT, 3, 4, GROUP, ZERO>(p, sms, dev, stream);
 }
 
 // Columns of a segment: 8, or 16 where an expert has more than 8 tokens on average (bf16 only: fp32's three terms
@@ -657,10 +608,9 @@ int hgemm_w4_moe(const void* x, int x_dtype, long long ldx, const int* ids, cons
     p.down = hgw::make_weight(down->q, down->scales, down->zeros, D, F, down->group);
     p.vec = !hgw::misaligned(x, 16) && D % 8 == 0 && p.ldx % (16 / size) == 0;
     const int held = (T < most ? T : most) * top_k;  // pairs of a launch
-    p.h = workspace;
+    p.h = static_cast<float*>(workspace);
     p.h_stride = static_cast<int>(hgw::padded_rows(F));
-    p.h_low = static_cast<long long>(held) * p.h_stride;
-    p.y = static_cast<float*>(workspace) + static_cast<size_t>(held) * p.h_stride;
+    p.y = p.h + static_cast<size_t>(held) * p.h_stride;
     p.y_stride = static_cast<int>(hgw::padded_rows(D));
     // Launches of up to kMaxTokens tokens; they share the workspace, in stream order.
     for (int t0 = 0; t0 < T; t0 += most) {

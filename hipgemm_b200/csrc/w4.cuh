@@ -176,7 +176,7 @@ struct RowSource<float> {
     __device__ __forceinline__ void load_full(Raw& raw, int k) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float4 f = __ldg(reinterpret_cast<const float4*>(row + k) + (i & 1) + 8 * (i / 2));
+            const float4 f = reinterpret_cast<const float4*>(row + k)[(i & 1) + 8 * (i / 2)];
             raw.v[4 * i] = f.x, raw.v[4 * i + 1] = f.y, raw.v[4 * i + 2] = f.z, raw.v[4 * i + 3] = f.w;
         }
     }
@@ -187,15 +187,15 @@ struct RowSource<float> {
             if (vec) {
                 float4 f0 = make_float4(0.f, 0.f, 0.f, 0.f), f1 = f0;
                 if (at < len) {
-                    f0 = __ldg(reinterpret_cast<const float4*>(row + at));
-                    f1 = __ldg(reinterpret_cast<const float4*>(row + at) + 1);
+                    f0 = reinterpret_cast<const float4*>(row + at)[0];
+                    f1 = reinterpret_cast<const float4*>(row + at)[1];
                 }
                 float* v = raw.v + 8 * h;
                 v[0] = f0.x, v[1] = f0.y, v[2] = f0.z, v[3] = f0.w;
                 v[4] = f1.x, v[5] = f1.y, v[6] = f1.z, v[7] = f1.w;
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) raw.v[8 * h + i] = at + i < len ? __ldg(row + at + i) : 0.0f;
+                for (int i = 0; i < 8; ++i) raw.v[8 * h + i] = at + i < len ? row[at + i] : 0.0f;
             }
         }
     }
@@ -204,13 +204,10 @@ struct RowSource<float> {
     __device__ __forceinline__ static void terms(const Raw& raw, uint32_t (&b)[3][8]) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            float x0 = raw.v[2 * i], x1 = raw.v[2 * i + 1];
-#pragma unroll
-            for (int s = 0; s < 3; ++s) {
-                b[s][i] = upper_halves(x0, x1);
-                x0 = after_bf16(x0);
-                x1 = after_bf16(x1);
-            }
+            const float x0 = raw.v[2 * i], x1 = raw.v[2 * i + 1], y0 = after_bf16(x0), y1 = after_bf16(x1);
+            b[0][i] = upper_halves(x0, x1);
+            b[1][i] = upper_halves(y0, y1);
+            b[2][i] = upper_halves(y0 - bf16_hi(__float_as_uint(y0)), y1 - bf16_hi(__float_as_uint(y1)));  // y is no infinity
         }
     }
 };
@@ -243,9 +240,10 @@ __device__ __forceinline__ void copy_wait() {
 
 constexpr int kStepK = 128;
 
-// DEEP loads x two tiles ahead instead of one: registers for latency.  For the experts, whose units are short, 15.7
-// us instead of 17.5 (one token) and 239 instead of 246 (32); for the linear kernel, which then fits an SM less
-// often, 38 instead of 34 (28672 x 8192 by 8 rows) and 54 instead of 47 (by 16).
+// DEEP loads x two tiles ahead instead of one: registers for latency.  For the experts' gate and up, whose units are
+// short, 15.7 us instead of 17.5 (one token) and 239 instead of 246 (32); for kernels that then fit an SM less often
+// it costs: the experts' down (three terms of fp32 a column) 19.4 instead of 18.0 and 314 instead of 289, the linear
+// kernel 38 instead of 34 (28672 x 8192 by 8 rows) and 54 instead of 47 (by 16).
 template <int R, int NT, int STAGES, int GROUP, bool ZERO, bool DEEP, typename Source>
 struct WarpProduct {
     static constexpr int kGroups = kStepK / GROUP;  // groups of a step

@@ -338,7 +338,7 @@ typedef struct {
  * gate and up: stacks of E (F x D) of the same group size, both with or both without zero
  * points; down: a stack of E (D x F).  An id outside [0, E) adds nothing (padding, experts of
  * another rank); an id that a token has twice counts with both weights.  Sums in fp32; the
- * product between the matrices is kept in 16 significant bits or more.  Codes of an expert are
+ * product between the matrices is kept in fp32.  Codes of an expert are
  * read once per 8 or 16 of its tokens; tokens beyond 64 (or 512 / top_k) take further launches.  The
  * result's bits depend on the inputs alone.
  * workspace: device memory, 16-byte aligned, hgemm_w4_moe_workspace_bytes(); its content does not
