@@ -553,16 +553,18 @@ constexpr int kRowsWarps = 16;
 
 template <typename T, int MT, int XS, int GROUP, bool ZERO>
 struct RowsShape {
-    // 10 KB of codes and scales a warp are in flight or in use: 160 KB an SM.
-    static constexpr int kOneStage = WarpStationary<T, MT, XS, 1, GROUP, ZERO>::kStageBytes;
-    static constexpr int kStages = 10240 / kOneStage;
+    using One = WarpStationary<T, MT, XS, 1, GROUP, ZERO>;
+    static constexpr int kBatch = MT == 0 ? 8 : 2;
+    static constexpr int kBatchFloats = kBatch * kRowsWarps * One::kResult;  // [row block][warp][kResult]
+    static constexpr int kExchange = kBatch * 16 * One::kColumns;       // a CTA's sums: [column][row block][row]
+    static constexpr int kSums = 2 * (kBatchFloats + kExchange) * 4;
+    // 10 KB of codes and scales a warp are in flight or in use, 160 KB an SM; less where x takes the room.
+    static constexpr int kRoom = (227 * 1024 - kSums) / kRowsWarps - (One::kWarpBytes - One::kStageBytes);
+    static constexpr int kStages = (kRoom < 10240 ? kRoom : 10240) / One::kStageBytes;
     static_assert(kStages >= 2, "a stage ahead");
     using Product = WarpStationary<T, MT, XS, kStages, GROUP, ZERO>;
-    static constexpr int kBatch = MT == 0 ? 8 : 2;
     static constexpr int kRings = kRowsWarps * Product::kWarpBytes;
-    static constexpr int kBatchFloats = kBatch * kRowsWarps * Product::kResult;  // [row block][warp][kResult]
-    static constexpr int kExchange = kBatch * 16 * Product::kColumns;       // a CTA's sums: [column][row block][row]
-    static constexpr int kSmem = kRings + 2 * (kBatchFloats + kExchange) * 4;
+    static constexpr int kSmem = kRings + kSums;
 };
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
@@ -725,18 +727,17 @@ int launch_rows(const LinearParams& p, const RowsPlan& plan, int dev, cudaStream
                           Shape::kSmem, stream, p);
 }
 
-// Most steps that a warp's registers take, by tiles of planes: 8 registers a step and tile.
-template <typename T, int MT>
+// Most steps that a warp's registers take: 8 registers a step and tile of planes.
+template <int MT>
 struct RowsLimits {
-    static constexpr int kTiles = MT == 0 ? 1 : MT * (sizeof(T) == 4 ? 4 : 3);
-    static_assert(kTiles <= 4, "16 warps leave 128 registers a thread");
-    static constexpr int kSteps = kTiles == 1 ? 4 : 2;
+    static_assert(MT <= 1, "16 warps leave 128 registers a thread");
+    static constexpr int kSteps = MT == 0 ? 4 : 2;
 };
 
 // False where the plan costs less than `least` (too little work to hold x for) or K is too long for the warps' registers.
 template <typename T, int MT, int GROUP, bool ZERO>
 bool run_rows(const LinearParams& p, int least, int sms, int dev, cudaStream_t stream, int* rc) {
-    using Limits = RowsLimits<T, MT>;
+    using Limits = RowsLimits<MT>;
     RowsPlan best;
     for (int split = 1; split <= 4; split *= 2) {
         const RowsPlan plan = rows_plan(p.w.row_blocks, ceil_div(p.w.k_blocks, 2), split, resident_clusters(split, sms, dev),

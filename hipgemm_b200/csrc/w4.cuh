@@ -408,17 +408,24 @@ struct WarpProduct {
 
 // ---- a warp's product with the activations held as whole numbers ---------------------------------
 //
-// For up to 16 rows of x the products above are bound by instructions: 28 logic instructions and 16
+// For few rows of x the products above are bound by instructions: 28 logic instructions and 16
 // subtractions per 512 bytes of codes to make bf16 of them.  As bytes the codes need 12: (w ^ 0x88..)
 // & 0xF0.. is 16 (code - 8) of the four high nibbles as signed bytes, and the same of w << 4 that of
 // the low ones; with integer tensor instructions the sums are exact as well.  So x is turned into
 // whole numbers, once: a warp keeps its K slice of x (XS steps of 128) in registers for all the row
-// blocks it goes through.  With 2^e the slice's scale, |x| < 2^e for all of a row's slice,
-//     x = 2^(e - 7) (i0 + 2^-7 i1 + 2^-14 i2 [+ 2^-21 i3]),   |i| <= 128
-// to half of the last place: 2^-21 of the slice's largest element from three planes (bf16), 2^-28
-// from four (fp32).  bf16 elements down to 2^-13 of the largest, and fp32 ones down to 2^-4, are
-// exact; of smaller ones so much is lost as fp32 sums lose that have the largest in them.  A slice
-// with an infinity, a NaN or an extreme exponent is computed from x itself (direct()).
+// blocks it goes through.  With 2^e just above the largest element of a row's slice, x = 2^(e - 31) n and the
+// bytes of n, each in -128..127, are four planes:
+//     n = 2^24 i0 + 2^16 i1 + 2^8 i2 + i3        (n + 0x808080, then the lower three bytes less 128).
+// Every element keeps its value whatever the largest is, since a row of W may have only zeros there:
+//   bf16: a slice with an element that is no multiple of the unit 2^(e - 31), for which it has to be below 2^(e - 24),
+//         is computed from x itself (direct());
+//   fp32: where an element is off by more than 2^-20 of itself, 2^8 (x / unit - n) is a fifth plane, kept in shared
+//         memory (of normally distributed x one slice of 512 elements in five has such an element); where that is
+//         not enough, direct().
+// direct() also takes slices with an infinity, a NaN or an extreme exponent.  A warp with the fifth plane issues a
+// quarter more matrix instructions (8192 x 8192 by 3 rows of fp32, every warp: 25.3 us instead of 19.6; that is why
+// not for 2^-24), one that takes direct() has twice the work (by 3 rows with nine elements of 1e5: 32 us;
+// 28672 x 8192 by one row of bf16 24.8 and 44).
 //
 // Columns: up to two rows of x take one tile, column 4 m + plane; else (fp32) plane p of 8 rows is
 // tile p, and the planes are put together in the same lane.
@@ -451,19 +458,25 @@ __device__ __forceinline__ float raw_element<__nv_bfloat16>(const RowSource<__nv
 // MT = 0: up to two rows of x in one tile; MT = 1: 8 rows, a tile a plane.
 template <typename T, int MT, int XS, int STAGES, int GROUP, bool ZERO>
 struct WarpStationary {
-    static constexpr bool kPacked = MT == 0;
+    static constexpr bool kPacked = MT == 0, kFifth = sizeof(T) == 4;
     static constexpr int kRowTiles = kPacked ? 1 : MT;
-    static constexpr int kPlanes = sizeof(T) == 4 ? 4 : 3;
-    static constexpr int kTiles = kPacked ? 1 : MT * kPlanes;  // tiles of plane columns
+    static constexpr int kPlanes = 4;
+    static constexpr int kTiles = kPacked ? 1 : MT * kPlanes;        // tiles of plane columns in registers
+    static constexpr int kAllTiles = kTiles + (kFifth ? kRowTiles : 0);  // and in shared memory
     static constexpr int kColumns = kPacked ? 2 : 8 * MT;
     static constexpr int kGroups = kStepK / GROUP;
     static constexpr int kCodes = XS * 2 * kTileBytes;
     static constexpr int kScales = XS * kGroups * 32;  // a group: 8 pairs of bf16, then (ZERO) 8 pairs of bytes
     static constexpr int kStageBytes = kCodes + (ZERO ? kScales * 3 / 2 : kScales);
-    static constexpr int kSumBytes = ZERO ? XS * kGroups * kTiles * 8 * 4 : 0;  // sums of x by group and column
-    static constexpr int kWarpBytes = kStageBytes * STAGES + kSumBytes;
+    static constexpr int kSumBytes = ZERO ? XS * kGroups * kAllTiles * 8 * 4 : 0;  // sums of x by group and column
+    // The fifth plane: B fragments, 8 bytes a lane, by 32 K; packed, of the 8 lanes that have columns 0 and 4.
+    static constexpr int kFifthWords = kPacked ? 16 : 64;
+    static constexpr int kFifthBytes = kFifth ? kRowTiles * XS * 4 * kFifthWords * 4 : 0;
+    static constexpr int kWarpBytes = kStageBytes * STAGES + kSumBytes + kFifthBytes;
     static constexpr int kSumStride = 20;  // floats from column to column of a warp's result: no bank conflicts
     static constexpr int kResult = kColumns * kSumStride;
+    // An element of fp32 x is off by no more than this part of itself.
+    static constexpr float kHeld = 0x1p-20f;
 
     struct Rows {
         RowSource<T> tile[kRowTiles];  // rows of x by B fragment column
@@ -471,15 +484,19 @@ struct WarpStationary {
     Rows x;
     uint32_t b[XS][4][kTiles][2];
     float factor[kRowTiles][2];      // 2^(e - 11) of columns 2 t, 2 t + 1 (of a plane's, if packed)
-    bool special;
+    bool special, fifth;             // computed from x itself; with the fifth plane
     int block0, blocks;              // K blocks of the slice
     uint8_t* ring;
     float* x_sums;
+    uint32_t* fifth_words;           // this lane's two of each 32 K, null if it has none
 
     // K blocks [first, first + 2 XS); those past `k_blocks` do not exist.
     __device__ __forceinline__ void set_slice(uint8_t* warp_smem, int first, int k_blocks, int lane) {
         ring = warp_smem;
         x_sums = reinterpret_cast<float*>(warp_smem + kStageBytes * STAGES);
+        fifth_words = reinterpret_cast<uint32_t*>(warp_smem + kStageBytes * STAGES + kSumBytes);
+        if (!kPacked) fifth_words += 2 * lane;
+        else fifth_words = lane / 4 % 4 == 0 ? fifth_words + 2 * (lane / 16 * 4 + lane % 4) : nullptr;
         block0 = first;
         blocks = min(2 * XS, max(0, k_blocks - first));
         // Scales that are never copied stand for groups past the end of a row.
@@ -489,14 +506,24 @@ struct WarpStationary {
         __syncwarp();
     }
 
+    // Four bytes, one of each y, in the codes' order in a word: k, k + 2, k + 1, k + 3.  `pick`: the byte as __byte_perm
+    // selects it from its first operand, and 16 times (4 more) for the second.
+    __device__ __forceinline__ static uint32_t gather(const uint32_t (&y)[4], uint32_t pick) {
+        return __byte_perm(__byte_perm(y[0], y[2], pick), __byte_perm(y[1], y[3], pick), 0x5410);
+    }
+
     // Turns the slice of x into planes.  `full_blocks`: K blocks loaded without a look at the row's end.
     __device__ __forceinline__ void convert(int full_blocks, int lane) {
-        special = false;
+        special = fifth = false;
         auto load = [&](typename RowSource<T>::Raw& raw, int m, int i) {
             if (block0 + i < full_blocks) x.tile[m].load_full(raw, (block0 + i) * kTileK);
             else x.tile[m].load(raw, (block0 + i) * kTileK);
         };
         typename RowSource<T>::Raw raw;
+        uint32_t lost = 0u;  // bf16: bits of what the planes do not hold
+        // Packed, lane 4 g + t has plane g % 4 of row g / 4.
+        const int plane = lane / 4 % 4;
+        const uint32_t pick = 0x73u - 0x11u * static_cast<uint32_t>(plane);
 #pragma unroll
         for (int m = 0; m < kRowTiles; ++m) {
             // Once for the largest element, once more (from L1) for the planes: the slice does not fit the registers.
@@ -513,17 +540,14 @@ struct WarpStationary {
                 const float other = __shfl_xor_sync(0xffffffffu, top, o);
                 asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(other));
             }
-            // top < 2^e, e = exponent - 126: x * 2^(7 - e) is below 128.
-            int exponent = static_cast<int>(__float_as_uint(top) >> 23);
-            special |= top != 0.0f && (exponent < 40 || exponent > 230);
-            exponent = min(max(exponent, 40), 230);
-            const float up = __uint_as_float(static_cast<uint32_t>(260 - exponent) << 23);     // 2^(133 - exponent)
-            float down = __uint_as_float(static_cast<uint32_t>(exponent - 10) << 23);          // 2^(exponent - 137): and 16 less
-            if (kPacked) {
-                // Lane 4 g + t has plane g % 4 of row g / 4; the factor is that of the plane.
-                const int plane = lane / 4 % 4;
-                down *= __uint_as_float(static_cast<uint32_t>(127 - 7 * plane) << 23);
-            }
+            // e = exponent - 126, with top below 2^e (1 - 2^-7): then n + 0x808080 does not overflow.  e <= 31, so that
+            // x * 2^(31 - e) is exact.
+            const uint32_t bits = __float_as_uint(top);
+            special |= bits != 0u && (bits < 50u << 23 || bits >= 157u << 23);
+            const int exponent = min(max(static_cast<int>((bits + 0x20000u) >> 23), 50), 157);
+            const float up = __uint_as_float(static_cast<uint32_t>(284 - exponent) << 23);     // 2^(31 - e)
+            float down = __uint_as_float(static_cast<uint32_t>(exponent - 10) << 23);          // 2^(e - 7), and 16 less
+            if (kPacked) down *= __uint_as_float(static_cast<uint32_t>(127 - 8 * plane) << 23);
 #pragma unroll
             for (int i = 0; i < 2; ++i) factor[m][i] = __shfl_sync(0xffffffffu, down, 4 * (2 * (lane & 3) + i));
 #pragma unroll
@@ -531,48 +555,68 @@ struct WarpStationary {
                 load(raw, m, i);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {  // 4 elements: one register of each plane
-                    float r[4];
+                    uint32_t y[4], z[4];
 #pragma unroll
-                    for (int l = 0; l < 4; ++l) r[l] = raw_element<T>(raw, 4 * j + l) * up;
-                    uint32_t mine = 0u;
-#pragma unroll
-                    for (int p = 0; p < kPlanes; ++p) {
-                        uint32_t n[4];
-#pragma unroll
-                        for (int l = 0; l < 4; ++l) {
-                            // 128 does not fit: 127, and the next plane has the rest.
-                            const float whole = fminf(r[l] + kMagic, kMagic + 127.0f);
-                            n[l] = __float_as_uint(whole);
-                            r[l] = (r[l] - (whole - kMagic)) * 128.0f;
+                    for (int l = 0; l < 4; ++l) {
+                        const float r = raw_element<T>(raw, 4 * j + l) * up;
+                        const int n = __float2int_rn(r);
+                        y[l] = (static_cast<uint32_t>(n) + 0x00808080u) ^ 0x00808080u;
+                        const float rest = r - __int2float_rn(n);  // exact: 0 from 2^23 on
+                        if constexpr (kFifth) {
+                            // 128 does not fit: 127, and what that leaves.
+                            const float whole = fminf(fmaf(rest, 256.0f, kMagic), kMagic + 127.0f);
+                            z[l] = __float_as_uint(whole);
+                            const float held = kHeld * fabsf(r);
+                            fifth |= fabsf(rest) > held;
+                            special |= fabsf(fmaf(whole - kMagic, -0x1p-8f, rest)) > held;
+                        } else {
+                            lost |= __float_as_uint(rest);
                         }
-                        // The codes' order in a word: k, k + 2, k + 1, k + 3.
-                        const uint32_t word = __byte_perm(__byte_perm(n[0], n[2], 0x0040), __byte_perm(n[1], n[3], 0x0040), 0x5410);
-                        if (kPacked) mine = p == lane / 4 % 4 ? word : mine;
-                        else b[i / 2][i % 2 * 2 + j / 2][m * kPlanes + p][j % 2] = word;
                     }
-                    if (kPacked) b[i / 2][i % 2 * 2 + j / 2][0][j % 2] = mine;
+                    if constexpr (kPacked) {
+                        b[i / 2][i % 2 * 2 + j / 2][0][j % 2] = gather(y, pick);
+                    } else {
+#pragma unroll
+                        for (int p = 0; p < kPlanes; ++p) b[i / 2][i % 2 * 2 + j / 2][m * kPlanes + p][j % 2] = gather(y, 0x73u - 0x11u * p);
+                    }
+                    if constexpr (kFifth) {
+                        const uint32_t word = gather(z, 0x40u);
+                        if (!kPacked || plane == 0) fifth_words[(m * XS * 4 + 2 * i + j / 2) * kFifthWords + j % 2] = word;
+                    }
                 }
             }
         }
-        special = __any_sync(0xffffffffu, special);
+        special = __any_sync(0xffffffffu, special || lost != 0u);
+        fifth = __any_sync(0xffffffffu, fifth);
         if (ZERO) {
             const uint32_t ones[4] = {0x10101010u, 0x10101010u, 0x10101010u, 0x10101010u};
 #pragma unroll
             for (int g = 0; g < XS * kGroups; ++g)
 #pragma unroll
-                for (int n = 0; n < kTiles; ++n) {
+                for (int n = 0; n < kAllTiles; ++n) {
                     int sum[4] = {0, 0, 0, 0};
 #pragma unroll
                     for (int c = 0; c < GROUP / 32; ++c) {
                         const int at = g * (GROUP / 32) + c;
-                        mma_s8(sum, ones, b[at / 4][at % 4][n][0], b[at / 4][at % 4][n][1], sum);
+                        if (n < kTiles) {
+                            mma_s8(sum, ones, b[at / 4][at % 4][n][0], b[at / 4][at % 4][n][1], sum);
+                        } else {
+                            const uint2 w = fifth_at(n - kTiles, at);
+                            mma_s8(sum, ones, w.x, w.y, sum);
+                        }
                     }
                     if (lane < 4)
-                        *reinterpret_cast<float2*>(x_sums + (g * kTiles + n) * 8 + 2 * lane) =
+                        *reinterpret_cast<float2*>(x_sums + (g * kAllTiles + n) * 8 + 2 * lane) =
                             make_float2(static_cast<float>(sum[0]), static_cast<float>(sum[1]));
                 }
             __syncwarp();
         }
+    }
+
+    // This lane's B fragment of the fifth plane, 32 K `k32` of the slice.
+    __device__ __forceinline__ uint2 fifth_at(int m, int k32) const {
+        if (kPacked && !fifth_words) return make_uint2(0u, 0u);
+        return *reinterpret_cast<const uint2*>(fifth_words + (m * XS * 4 + k32) * kFifthWords);
     }
 
     // Starts the copies of the slice of one row block.  q: this lane's 16 bytes of the row block's first tile; scales,
@@ -597,13 +641,22 @@ struct WarpStationary {
         const uint8_t* in = ring + stage * kStageBytes;
         if (special) {
             direct(in, x, block0, blocks, result, lane);
-            return;
+        } else if (kFifth && fifth) {
+            products<kFifth>(in, flip, high, result, lane);
+        } else {
+            products<false>(in, flip, high, result, lane);
         }
+    }
+
+private:
+    template <bool FIFTH>
+    __device__ __forceinline__ void products(const uint8_t* in, uint32_t flip, uint32_t high, float* result, int lane) const {
         float acc[kRowTiles][4];
 #pragma unroll
         for (int m = 0; m < kRowTiles; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.0f;
         const int magic[4] = {kMagicBits, kMagicBits, kMagicBits, kMagicBits};
-        int sum[kTiles][4];
+        constexpr int kUsed = FIFTH ? kAllTiles : kTiles;
+        int sum[kUsed][4];
 #pragma unroll
         for (int i = 0; i < 2 * XS; ++i) {
             const uint4 codes = *reinterpret_cast<const uint4*>(in + i * kTileBytes + lane * 16);
@@ -620,12 +673,20 @@ struct WarpStationary {
                 const int k32 = 2 * i + h;  // of the slice
                 const bool first = k32 * 32 % GROUP == 0, last = (k32 + 1) * 32 % GROUP == 0;
 #pragma unroll
-                for (int n = 0; n < kTiles; ++n)
-                    {
-                    if (first) mma_s8(sum[n], a, b[i / 2][k32 % 4][n][0], b[i / 2][k32 % 4][n][1], magic);
-                    else mma_s8(sum[n], a, b[i / 2][k32 % 4][n][0], b[i / 2][k32 % 4][n][1], sum[n]);
+                for (int n = 0; n < kUsed; ++n) {
+                    uint32_t b0, b1;
+                    if (n < kTiles) {
+                        b0 = b[i / 2][k32 % 4][n][0];
+                        b1 = b[i / 2][k32 % 4][n][1];
+                    } else {
+                        const uint2 w = fifth_at(n - kTiles, k32);
+                        b0 = w.x;
+                        b1 = w.y;
+                    }
+                    if (first) mma_s8(sum[n], a, b0, b1, magic);
+                    else mma_s8(sum[n], a, b0, b1, sum[n]);
                 }
-                if (last) flush(in, k32 * 32 / GROUP, sum, acc, lane);
+                if (last) flush<FIFTH>(in, k32 * 32 / GROUP, sum, acc, lane);
             }
         }
         if (kPacked) {
@@ -643,9 +704,9 @@ struct WarpStationary {
         }
     }
 
-private:
     // acc += scale * 2^(e - 7) * sum over the group of (code - zero) * (the planes).
-    __device__ __forceinline__ void flush(const uint8_t* in, int group, const int (&sum)[kTiles][4], float (&acc)[kRowTiles][4],
+    template <bool FIFTH, int USED>
+    __device__ __forceinline__ void flush(const uint8_t* in, int group, const int (&sum)[USED][4], float (&acc)[kRowTiles][4],
                                           int lane) const {
         const uint32_t pair = *reinterpret_cast<const uint32_t*>(in + kCodes + group * 32 + lane / 4 * 4);
         const float scale[2] = {bf16_lo(pair), bf16_hi(pair)};
@@ -656,23 +717,29 @@ private:
             shift[0] = (8388608.0f + 8.0f) - __uint_as_float(__byte_perm(z, 0x4B000000u, 0x7550));
             shift[1] = (8388608.0f + 8.0f) - __uint_as_float(__byte_perm(z, 0x4B000000u, 0x7551));
         }
+        // A plane's sums, whole numbers below 2^23.
+        auto whole = [&](int n, int i) {
+            float u = __int_as_float(sum[n][i]) - kMagic;
+            if (ZERO) {
+                const float2 sums = *reinterpret_cast<const float2*>(x_sums + (group * kAllTiles + n) * 8 + 2 * (lane & 3));
+                u = fmaf(shift[i / 2], i % 2 ? sums.y : sums.x, u);
+            }
+            return u;
+        };
 #pragma unroll
         for (int m = 0; m < kRowTiles; ++m) {
-            float v[4];
 #pragma unroll
-            for (int p = kPacked ? 0 : kPlanes - 1; p >= 0; --p) {
-                const int n = kPacked ? 0 : m * kPlanes + p;
-                float2 sums;
-                if (ZERO) sums = *reinterpret_cast<const float2*>(x_sums + (group * kTiles + n) * 8 + 2 * (lane & 3));
+            for (int i = 0; i < 4; ++i) {
+                // Packed, the fifth plane lies in the first one's column, and the others add up across lanes.
+                float v = 0.0f;
+                if (FIFTH) v = kPacked ? whole(kTiles + m, i) * 0x1p-24f : whole(kTiles + m, i);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float u = __int_as_float(sum[n][i]) - kMagic;
-                    if (ZERO) u = fmaf(shift[i / 2], i % 2 ? sums.y : sums.x, u);
-                    v[i] = kPacked || p == kPlanes - 1 ? u : fmaf(v[i], 0x1p-7f, u);
+                for (int p = kPacked ? 0 : kPlanes - 1; p >= 0; --p) {
+                    const float u = whole(kPacked ? 0 : m * kPlanes + p, i);
+                    v = FIFTH || (!kPacked && p < kPlanes - 1) ? fmaf(v, 0x1p-8f, u) : u;
                 }
+                acc[m][i] = fmaf(scale[i / 2], v * factor[m][i % 2], acc[m][i]);
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[m][i] = fmaf(scale[i / 2], v[i] * factor[m][i % 2], acc[m][i]);
         }
     }
 

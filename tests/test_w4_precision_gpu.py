@@ -51,3 +51,74 @@ def test_experts_keep_the_product_between_the_matrices(cuda_device, t, group, ze
     off = want.abs() * 2.0 ** -20 + size * (2.0 ** -24 + 6 * ref.ADD)
     got = hg.w4_moe(x.to(dtype).cuda(), torch.zeros(t, 1, dtype=torch.int32).cuda(), torch.ones(t, 1).cuda(), wg, wu, wd)
     ref.assert_close(got, want, off, dtype)
+
+
+# ---- rows held in registers as whole numbers ------------------------------------------------------
+#
+# One or two rows, and any fp32 rows, of matrices that are large enough.
+
+ROWS = [(1, torch.bfloat16), (2, torch.bfloat16), (1, torch.float32), (2, torch.float32), (3, torch.float32),
+        (8, torch.float32), (11, torch.float32)]
+ROW_IDS = [f"{m}-{str(t).split('.')[1]}" for m, t in ROWS]
+TERMS = {torch.bfloat16: 1, torch.float32: 3}
+
+
+@pytest.mark.parametrize("m,dtype", ROWS, ids=ROW_IDS)
+@pytest.mark.parametrize("n,k,group,zero_point", [(5120, 1024, 128, False), (7100, 1100, 32, True), (2500, 4000, 64, True),
+                                                  (4096, 2113, 128, True)])
+def test_an_element_keeps_its_value_beside_any_other(cuda_device, m, n, k, group, zero_point, dtype):
+    """Row r of W is 1 at column r % K and 0 elsewhere: y has the elements of x, whose magnitudes are far apart."""
+    gen = _gen(m, n, k, group)
+    row = torch.arange(n)
+    zero = torch.randint(0, 15, (n, 1), generator=gen) if zero_point else torch.full((n, 1), 8)
+    codes = zero.expand(n, k).clone()
+    codes[row, row % k] += 1
+    groups = -(-k // group)
+    w = hg.w4_pack(codes.to(torch.uint8).cuda(), torch.ones(n, groups).cuda(),
+                   zero.expand(n, groups).to(torch.uint8).contiguous().cuda() if zero_point else None, group=group)
+    for lo, hi in [(0, 1), (-8, 8), (-24, 2), (-40, 20), (-50, 60)]:
+        x = (torch.randn(m, k, generator=gen) * torch.exp2(torch.randint(lo, hi, (m, k), generator=gen).float())).to(dtype)
+        got = hg.w4_gemm_tn(x.cuda(), w).cpu()
+        want = x[:, row % k]
+        if dtype == torch.bfloat16:
+            assert torch.equal(got, want)
+        else:
+            # An element is held to 2^-20 of itself; five planes, put together in four additions.
+            assert bool(((got.double() - want.double()).abs() <= want.double().abs() * (2.0 ** -20 + 4 * 2.0 ** -24)).all())
+
+
+@pytest.mark.parametrize("m,dtype", ROWS, ids=ROW_IDS)
+@pytest.mark.parametrize("zero_point", [False, True])
+@pytest.mark.parametrize("size", [1.0e4, 1.0e5, 2.0 ** 20, 2.0 ** 40])
+def test_an_outlier_that_no_weight_meets_costs_nothing(cuda_device, m, dtype, zero_point, size):
+    gen = _gen(m, int(size) % 1000, 5)
+    n, k, group = 5120, 2048, 64
+    codes, scales, zeros = ref.random_weight(gen, (n, k), group, zero_point)
+    at = torch.randint(0, k, (9,), generator=gen)
+    codes[:, at] = 8 if zeros is None else zeros[:, at // group]
+    w = hg.w4_pack(codes.cuda(), scales.cuda(), None if zeros is None else zeros.cuda(), group=group)
+    values = ref.values(codes, scales, zeros, group)
+    x = torch.randn(m, k, generator=gen)
+    x[:, at] = size * torch.randn(m, 9, generator=gen)
+    x = x.to(dtype)
+    got = hg.w4_gemm_tn(x.cuda(), w)
+    want, off = ref.linear(x, values, TERMS[dtype])
+    ref.assert_close(got, want, off, dtype)
+    # The same row among others, which another kernel takes for bf16: each is off by its bound at most.
+    more = hg.w4_gemm_tn(torch.cat([x, x[:1], x[:1]]).cuda(), w)
+    ref.assert_close(more[:m], want, off, dtype)
+    bound = 2 * (off + ref.half_step(dtype) * (want.abs() + off))
+    assert bool(((more[:m].cpu().double() - got.cpu().double()).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("m,dtype", ROWS, ids=ROW_IDS)
+@pytest.mark.parametrize("n,k,group,zero_point", [(5120, 1024, 128, False), (7100, 1100, 32, True), (300, 20000, 64, False)])
+def test_weights_that_meet_the_small_elements_alone(cuda_device, m, n, k, group, zero_point, dtype):
+    gen = _gen(m, n, k, 9)
+    codes, scales, zeros = ref.random_weight(gen, (n, k), group, zero_point)
+    x = (torch.randn(m, k, generator=gen) * torch.exp2(torch.randint(-30, 1, (1, k), generator=gen).float())).to(dtype)
+    large = x.abs().amax(0) > 2.0 ** -20
+    none = torch.full((n, k), 8, dtype=torch.uint8) if zeros is None else zeros.repeat_interleave(group, 1)[:, :k]
+    codes = torch.where(large, none, codes)
+    w = hg.w4_pack(codes.cuda(), scales.cuda(), None if zeros is None else zeros.cuda(), group=group)
+    ref.assert_close(hg.w4_gemm_tn(x.cuda(), w), *ref.linear(x, ref.values(codes, scales, zeros, group), TERMS[dtype]), dtype)
