@@ -540,14 +540,15 @@ int launch_linear(const LinearParams& p, int sms, int dev, cudaStream_t stream) 
                           Shape::kSmem, stream, p);
 }
 
-// ---- the same for up to 16 rows, x held in registers -------------------------------------------
+// ---- the same for one or two rows, or rows of fp32, x held in registers ---------------------------
 //
 // A persistent grid, one CTA an SM: a cluster of `split` CTAs takes a range of row blocks, its warps
 // a slice of K each for all of them, so that x is read and turned into whole numbers once per warp
 // and codes are all that streams: 62 instructions a tile instead of 88.  28672 x 8192 by one row takes
-// 25.6 us (4.7 TB/s) instead of 34; what is left is start and end (4.8 us for 7168 x 2048, most of it
-// launch, the planes and the first bytes' latency).  After every kBatch row blocks the warps' sums are added up in
-// shared memory, then the CTAs' in distributed shared memory, in a fixed order.
+// 24.8 us (4.9 TB/s) instead of 34; what is left is start and end (4.5 us for 7168 x 2048, most of it
+// launch, the planes and the first bytes' latency).  W is read once per two rows, or 8 of fp32.  After
+// every kBatch row blocks the warps' sums are added up in shared memory, then the CTAs' in distributed
+// shared memory, in a fixed order.
 
 constexpr int kRowsWarps = 16;
 
@@ -760,14 +761,14 @@ int run_linear(const LinearParams& p, int sms, int dev, cudaStream_t stream) {
     int rc = 0;
     if constexpr (sizeof(T) == 4) {
         // Three matrix instructions for the three terms of x, and making the terms: x held in registers is faster nearly
-        // throughout (us here and there: 8192 x 8192 by 1 row 14.5 and 30.7, by 3 rows 19.4 and 31.2, by 16 39 and
+        // throughout (us here and there: 8192 x 8192 by 1 row 12.6 and 30.7, by 3 rows 19.6 and 31.2, by 16 45 and
         // 57; 4096 x 1024 by 3 4.7 and 6.7), but for the least work (1024 x 1024 by 1: 3.6 and 3.1).
         if (p.M <= 2 ? run_rows<T, 0, GROUP, ZERO>(p, 4, sms, dev, stream, &rc) : run_rows<T, 1, GROUP, ZERO>(p, 4, sms, dev, stream, &rc))
             return rc;
         return launch_linear<T, 2, 1, 3, GROUP, ZERO, 4>(p, sms, dev, stream);
     } else {
-        // One or two rows: x held in registers pays where there is work enough (us here and there: 28672 x 8192 25.6 and
-        // 34.3, 7168 x 2048 4.8 and 5.6, 4096 x 1024 3.9 and 2.8).  Three to eight rows take three times the integer
+        // One or two rows: x held in registers pays where there is work enough (us here and there: 28672 x 8192 24.8 and
+        // 34.3, 7168 x 2048 4.5 and 5.6, 4096 x 1024 3.9 and 2.8).  Three to eight rows take three times the integer
         // instructions: 8192 x 8192 16.5 and 12.7.
         if (p.M <= 2 && run_rows<T, 0, GROUP, ZERO>(p, 6, sms, dev, stream, &rc)) return rc;
         // The tensor cores from 17 rows on (us below and there, at 8192 x 8192 and at 28672 x 8192): 16 rows 14.8 and 14.5,

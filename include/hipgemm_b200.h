@@ -305,9 +305,10 @@ int hgemm_dequantize_w4(const void* q, const void* scales, const void* zeros, in
 
 /* y[M x N] = x[M x K] . W[N x K]^T for few rows of x (decoding): x fp32 or bf16 with `ldx`
  * elements from row to row, y row-major of the same type, sums in fp32, one rounding.  x is used
- * in full, except that for one or two rows, and for rows of fp32, it may be held in fixed point
- * against the largest element of up to 512 consecutive K of its row: to half of 2^-21 (bf16) or
- * 2^-28 (fp32) of that.  Any N and K, M <= 524280 (HGEMM_ERR_UNSUPPORTED above); y is fully
+ * in full, except that an element of fp32 x may be held to 2^-20 of itself, whatever lies beside
+ * it.  (One or two rows, and rows of fp32, are held as whole numbers; where elements of up to 512
+ * consecutive K lie more than about 2^24 (bf16) or 2^19 (fp32) apart, the call takes up to twice as
+ * long.)  Any N and K, M <= 524280 (HGEMM_ERR_UNSUPPORTED above); y is fully
  * overwritten; K == 0 writes zeros.  W is read once per 8 rows of fp32 or 16 to 64 of bf16 x, so
  * for many rows dequantise it instead.  The result's bits depend on the inputs alone.  Needs no
  * workspace.  x, y aligned to their element.  The first call on a device, outside any stream
