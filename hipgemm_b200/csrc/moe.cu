@@ -55,17 +55,17 @@ template <typename T>
 struct RouteLoad {
     static constexpr int kElements = 16 / sizeof(T);
     uint4 v;
-    __device__ __forceinline__ void load_full(const T* row, int at) { v = __ldg(reinterpret_cast<const uint4*>(row + at)); }
+    __device__ __forceinline__ void load_full(const T* row, int at) { v = *reinterpret_cast<const uint4*>(row + at); }
     __device__ __forceinline__ void load(const T* row, int at, int len, bool vec) {
         v = make_uint4(0u, 0u, 0u, 0u);
         if (vec) {
-            if (at < len) v = __ldg(reinterpret_cast<const uint4*>(row + at));
+            if (at < len) v = *reinterpret_cast<const uint4*>(row + at);
         } else {
             uint32_t e[kElements];
 #pragma unroll
             for (int i = 0; i < kElements; ++i) {
                 if constexpr (sizeof(T) == 4) e[i] = at + i < len ? __float_as_uint(row[at + i]) : 0u;
-                else e[i] = at + i < len ? __ldg(reinterpret_cast<const unsigned short*>(row + at + i)) : 0u;
+                else e[i] = at + i < len ? *reinterpret_cast<const unsigned short*>(row + at + i) : 0u;
             }
             if constexpr (sizeof(T) == 4) v = make_uint4(e[0], e[1], e[2], e[3]);
             else v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);

@@ -88,11 +88,11 @@ __device__ __forceinline__ void load8(const T* row, int at, int len, float (&v)[
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = 0.0f;
     } else if constexpr (sizeof(T) == 4) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(row + at));
-        const float4 b = __ldg(reinterpret_cast<const float4*>(row + at) + 1);
+        const float4 a = *reinterpret_cast<const float4*>(row + at);
+        const float4 b = reinterpret_cast<const float4*>(row + at)[1];
         v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
     } else {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + at));
+        const uint4 u = *reinterpret_cast<const uint4*>(row + at);
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -173,10 +173,9 @@ __device__ __forceinline__ void encode8(const float (&w0)[8], const float (&w1)[
 // 28672 x 8192 bf16 to codes and back takes 241 us, 4.9 TB/s of the two kernels' traffic (a division an
 // element made it 697); 4999 x 5115 fp32, whose rows go through shared memory, 72 us (scalar loads 211).
 template <typename T, bool ZERO, int GROUP, bool VEC>
-__global__ void __launch_bounds__(kQuantThreads) quantize_w4_kernel(const T* __restrict__ w, int N, int K, int row_blocks,
-                                                                    int k_blocks, int groups, unsigned items,
-                                                                    uint8_t* __restrict__ q, uint32_t* __restrict__ scales,
-                                                                    uint16_t* __restrict__ zeros) {
+__global__ void __launch_bounds__(kQuantThreads) quantize_w4_kernel(const T* w, int N, int K, int row_blocks, int k_blocks,
+                                                                    int groups, unsigned items, uint8_t* q,
+                                                                    uint32_t* scales, uint16_t* zeros) {
     __shared__ T staged[QuantSmem<T, VEC>::kElements];
     constexpr int kGroups = 128 / GROUP, kParts = GROUP / 32;
     const int lane = threadIdx.x & 31, g = lane / 4, t = lane & 3;
@@ -303,11 +302,10 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_w4_kernel(const T* __r
 // For bf16 the codes are unpacked as the products do it, two at a time, and multiplied by the
 // scale in bf16, which rounds the exact product once: the same value.
 template <typename T, bool ZERO, bool VEC>
-__global__ void __launch_bounds__(kQuantThreads) dequantize_w4_kernel(const uint8_t* __restrict__ q,
-                                                                      const uint32_t* __restrict__ scales,
-                                                                      const uint16_t* __restrict__ zeros, int N, int K,
+__global__ void __launch_bounds__(kQuantThreads) dequantize_w4_kernel(const uint8_t* q, const uint32_t* scales,
+                                                                      const uint16_t* zeros, int N, int K,
                                                                       int row_blocks, int k_blocks, int groups,
-                                                                      int group_shift, unsigned items, T* __restrict__ w) {
+                                                                      int group_shift, unsigned items, T* w) {
     __shared__ T staged[QuantSmem<T, VEC>::kElements];
     const int lane = threadIdx.x & 31, g = lane / 4, t = lane & 3;
     const unsigned warps = gridDim.x * kQuantWarps;
@@ -325,13 +323,19 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_w4_kernel(const uint
         const int left = K - kb * kTileK;
         T* tile = staged + threadIdx.x / 32 * (VEC ? 0 : 16 * kPitch);
         if (!VEC) __syncwarp();
+        uint32_t half_scales[2], half_zeros[2];  // of both halves before the first store
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const int k0 = 32 * c + 8 * t;
             int group = (kb * kTileK + 32 * c) >> group_shift;
             group = group < groups ? group : groups - 1;
             const size_t at = (static_cast<size_t>(block) * groups + group) * 8 + g;
-            const uint32_t sc = __ldg(scales + at), z = ZERO ? __ldg(zeros + at) : 0x0808u;
+            half_scales[c] = scales[at];
+            half_zeros[c] = ZERO ? zeros[at] : 0x0808u;
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int k0 = 32 * c + 8 * t;
+            const uint32_t sc = half_scales[c], z = half_zeros[c];
             uint32_t a[2][4];
 #pragma unroll
             for (int j = 0; j < 2; ++j)

@@ -95,10 +95,14 @@ __device__ __forceinline__ void unpack(uint32_t w, const UnpackConstants& c, uin
     }
 }
 
+// Loads: these kernels may start while the one before them on the stream still runs (see launch()), which may be what
+// writes their operands.  So they use ordinary loads after griddepcontrol.wait and none of the non-coherent path
+// (ld.global.nc, __ldg, const __restrict__), whose data has to be unchanged for the whole kernel.
+
 // A streaming 16-byte load: each weight byte is used once per call.
 __device__ __forceinline__ uint4 load_stream(const uint8_t* p) {
     uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                  : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                  : "l"(p));
     return v;
@@ -126,7 +130,7 @@ struct RowSource<__nv_bfloat16> {
     bool vec;  // rows 16-byte aligned and of a multiple of 8 elements
     __device__ __forceinline__ void load_full(Raw& raw, int k) const {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) raw.v[h] = __ldg(reinterpret_cast<const uint4*>(row + k) + 4 * h);
+        for (int h = 0; h < 2; ++h) raw.v[h] = reinterpret_cast<const uint4*>(row + k)[4 * h];
     }
     __device__ __forceinline__ void load(Raw& raw, int k) const {
 #pragma unroll
@@ -134,12 +138,12 @@ struct RowSource<__nv_bfloat16> {
             const int at = k + 32 * h;
             raw.v[h] = make_uint4(0u, 0u, 0u, 0u);
             if (vec) {
-                if (at < len) raw.v[h] = __ldg(reinterpret_cast<const uint4*>(row + at));
+                if (at < len) raw.v[h] = *reinterpret_cast<const uint4*>(row + at);
             } else {
                 uint32_t e[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    e[i] = at + i < len ? __ldg(reinterpret_cast<const unsigned short*>(row + at + i)) : 0u;
+                    e[i] = at + i < len ? *reinterpret_cast<const unsigned short*>(row + at + i) : 0u;
                 raw.v[h] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
             }
         }

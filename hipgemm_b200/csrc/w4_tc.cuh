@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(TcShape<NC>::kWarps * 32, 1) w4_tc_kernel(cons
 #pragma unroll
             for (int i = 0; i < kMine; ++i) {
                 const int group = (first + s) * kGroups + S::kFlushTeams * i + team;
-                next[i] = group < p.w.groups ? __ldg(scales + static_cast<size_t>(group) * 16) : 0u;
+                next[i] = group < p.w.groups ? scales[static_cast<size_t>(group) * 16] : 0u;
             }
         };
         load_scales(0);
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(TcShape<NC>::kWarps * 32, 1) w4_tc_kernel(cons
             for (int half = 0; half < 2; ++half)
 #pragma unroll
                 for (int i = 0; i < kGroups; ++i)
-                    next[half][i] = __ldg(zeros[half] + static_cast<size_t>(min((first + s) * kGroups + i, p.w.groups - 1)) * 8);
+                    next[half][i] = zeros[half][static_cast<size_t>(min((first + s) * kGroups + i, p.w.groups - 1)) * 8];
         };
 #pragma unroll
         for (int v = 0; v < S::kAhead; ++v) copy(team + S::kTeams * v, v);

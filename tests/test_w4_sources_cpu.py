@@ -1,0 +1,20 @@
+"""Rules that the sources of the 4-bit weight kernels keep and that no run can show to be broken."""
+import os
+import re
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "hipgemm_b200", "csrc")
+KERNELS = ["w4.cu", "w4.cuh", "w4_tc.cu", "w4_tc.cuh", "moe.cu"]
+
+
+def _code(name):
+    with open(os.path.join(CSRC, name)) as f:
+        return re.sub(r"//[^\n]*", "", f.read())
+
+
+@pytest.mark.parametrize("name", KERNELS)
+def test_no_non_coherent_loads(name):
+    """These kernels are launched with programmatic stream serialization: the kernel before them may be writing their
+    operands when they start, so that no load may take the path for data that never changes while a kernel runs."""
+    assert re.findall(r"__ldg|ld\.global[.\w:]*\.nc|\btex1D|__restrict__|__restrict\b", _code(name)) == []
