@@ -30,8 +30,11 @@ constexpr int kMaxSegments = kMaxPairs;
 //
 // A cluster of 8 CTAs takes TT tokens; its warps, in pairs that take half of D each, split the
 // experts, EW at a time, so that a load of x serves EW experts and one of the router TT tokens.
-// Sixteen products a lane are summed in fp32 and then added in 64 bits, so that experts whose logits
-// are close are ordered as the exact logits are.  The logits go to the CTA that selects the
+// Sixteen products a lane are summed in fp32 and then added in 64 bits: a logit is off by 16 roundings at
+// most, 16 * 2^-24 of the sum of |x r|, and experts whose logits are nearer than twice that may change
+// places (equal rows of the router never do: their sums have the same bits).  64 bits throughout took 50.8
+// us where this takes 32.5, and 7.1 where this takes 5.8; telling the close ones by a bound of |x| |r| and
+// summing those again 45 and 8.3.  The logits go to the CTA that selects the
 // token's experts over distributed shared memory.  Bound by the latency of the router's loads, all of
 // which each cluster reads from L2: hence two loads of each row at a time, in a branch without other
 // conditions (64 tokens, 7168 x 256 fp32: 32.5 us, 48 with a condition a load), and two CTAs an SM.

@@ -320,7 +320,10 @@ int hgemm_w4_gemm_tn(const void* x, int x_dtype, long long ldx, const void* q, c
 
 /* The router of a mixture of experts: logits = x[T x D] . router[E x D]^T (both of x_dtype),
  * p = softmax over all E, and per token the top_k largest: ids (T x top_k, largest first, ties to
- * the lower index, NaN last) and weights (p of those, divided by their sum if renormalize).
+ * the lower index, NaN last) and weights (p of those, divided by their sum if renormalize).  A
+ * logit is off by at most 2^-20 of the sum of |x router| (sums of 16 products in fp32, which have
+ * to be in its range, the rest in 64 bits), so that experts whose logits are nearer than twice that
+ * may change places; experts with equal rows tie.
  * E <= 1024 and top_k <= 16, else HGEMM_ERR_UNSUPPORTED.  Needs no workspace. */
 int hgemm_moe_route(const void* x, int x_dtype, long long ldx, const void* router, int T, int D, int E, int top_k,
                     int renormalize, int* ids, float* weights, hgemm_stream_t stream);
