@@ -71,6 +71,7 @@ _SIGNATURES = {
     "hgemm_quantize_w4": (_i, [_vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
     "hgemm_dequantize_w4": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _i, _vp]),
     "hgemm_w4_gemm_tn": (_i, [_vp, _i, ctypes.c_longlong, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "hgemm_debug_stalled_w4": (_i, [_vp, ctypes.c_longlong, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "hgemm_moe_route": (_i, [_vp, _i, ctypes.c_longlong, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp]),
     "hgemm_w4_moe": (_i, [_vp, _i, ctypes.c_longlong, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp,
                           ctypes.c_size_t, _vp]),

@@ -446,6 +446,7 @@ struct LinearParams {
     int M, N, K;
     Weight w;
     bool vec;
+    bool stall;  // hgemm_debug_stalled_w4
 };
 
 template <typename T>
@@ -757,8 +758,8 @@ bool run_rows(const LinearParams& p, int least, int sms, int dev, cudaStream_t s
 }
 
 // w4_tc.cu
-int run_tc(const void* x, long long ldx, void* y, int M, int N, int K, const Weight& w, int group, int sms, int dev,
-           cudaStream_t stream);
+int run_tc(const void* x, long long ldx, void* y, int M, int N, int K, const Weight& w, int group, bool stall, int sms,
+           int dev, cudaStream_t stream);
 
 template <typename T, int GROUP, bool ZERO>
 int run_linear(const LinearParams& p, int sms, int dev, cudaStream_t stream) {
@@ -778,7 +779,7 @@ int run_linear(const LinearParams& p, int sms, int dev, cudaStream_t stream) {
         // The tensor cores from 17 rows on (us below and there, at 8192 x 8192 and at 28672 x 8192): 16 rows 14.8 and 14.5,
         // 46.4 and 43.2, but 5.6 and 7.4 at 4096 x 4096; 17 rows 28.5 and 16.7, 86.4 and 51.7; 64 rows 44.3 and
         // 21.7, 153 and 68.2.
-        if (p.M > 16 && p.vec) return run_tc(p.x, p.ldx, p.y, p.M, p.N, p.K, p.w, GROUP, sms, dev, stream);
+        if (p.M > 16 && p.vec) return run_tc(p.x, p.ldx, p.y, p.M, p.N, p.K, p.w, GROUP, p.stall, sms, dev, stream);
         if (p.M <= 8) return launch_linear<T, 2, 1, 3, GROUP, ZERO, 8>(p, sms, dev, stream);
         if (p.M <= 16) return launch_linear<T, 2, 2, 3, GROUP, ZERO, 4>(p, sms, dev, stream);
         return launch_linear<T, 2, 4, 3, GROUP, ZERO, 4>(p, sms, dev, stream);
@@ -794,6 +795,41 @@ inline int check_weight(const void* q, const void* scales, const void* zeros, un
 }
 
 }  // namespace hgw
+
+namespace {
+
+int gemm_w4(const void* x, int x_dtype, long long ldx, const void* q, const void* scales, const void* zeros, void* y, int M,
+            int N, int K, int group, bool stall, hgemm_stream_t stream) {
+    if (M < 0 || N < 0 || K < 0 || !hgw::valid_group(group)) return HGEMM_ERR_INVALID_VALUE;
+    if (x_dtype != HGEMM_DTYPE_F32 && x_dtype != HGEMM_DTYPE_BF16) return HGEMM_ERR_INVALID_VALUE;
+    if (M > 1 && ldx < K) return HGEMM_ERR_INVALID_VALUE;
+    if (M == 0 || N == 0) return HGEMM_OK;
+    if (!y) return HGEMM_ERR_INVALID_VALUE;
+    const unsigned size = x_dtype == HGEMM_DTYPE_F32 ? 4 : 2;
+    if (hgw::misaligned(y, size)) return HGEMM_ERR_ALIGNMENT;
+    const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    int sms = 0, dev = 0;
+    if (K == 0) {
+        if (int rc = hgw::current_device(&sms, &dev)) return rc;
+        const size_t bytes = static_cast<size_t>(M) * N * size;
+        return cudaMemsetAsync(y, 0, bytes, s) == cudaSuccess ? HGEMM_OK : HGEMM_ERR_CUDA;
+    }
+    if (!x) return HGEMM_ERR_INVALID_VALUE;
+    if (int rc = hgw::check_weight(q, scales, zeros, 16)) return rc;
+    if (hgw::misaligned(x, size)) return HGEMM_ERR_ALIGNMENT;
+    if (int rc = hgw::current_device(&sms, &dev)) return rc;
+    if (M > 65535 * 8) return HGEMM_ERR_UNSUPPORTED;  // grid.y
+    hgw::LinearParams p{x, M > 1 ? ldx : 0, y, M, N, K, hgw::make_weight(q, scales, zeros, N, K, group),
+                        !hgw::misaligned(x, 16) && K % 8 == 0 && (M == 1 || ldx % (16 / size) == 0), stall};
+    return hgw::with_format(group, zeros != nullptr, [&](auto g, auto z) {
+        constexpr int G = decltype(g)::value;
+        constexpr bool Z = decltype(z)::value;
+        return x_dtype == HGEMM_DTYPE_F32 ? hgw::run_linear<float, G, Z>(p, sms, dev, s)
+                                          : hgw::run_linear<__nv_bfloat16, G, Z>(p, sms, dev, s);
+    });
+}
+
+}  // namespace
 
 extern "C" {
 
@@ -845,33 +881,14 @@ int hgemm_dequantize_w4(const void* q, const void* scales, const void* zeros, in
 
 int hgemm_w4_gemm_tn(const void* x, int x_dtype, long long ldx, const void* q, const void* scales, const void* zeros,
                      void* y, int M, int N, int K, int group, hgemm_stream_t stream) {
-    if (M < 0 || N < 0 || K < 0 || !hgw::valid_group(group)) return HGEMM_ERR_INVALID_VALUE;
-    if (x_dtype != HGEMM_DTYPE_F32 && x_dtype != HGEMM_DTYPE_BF16) return HGEMM_ERR_INVALID_VALUE;
-    if (M > 1 && ldx < K) return HGEMM_ERR_INVALID_VALUE;
-    if (M == 0 || N == 0) return HGEMM_OK;
-    if (!y) return HGEMM_ERR_INVALID_VALUE;
-    const unsigned size = x_dtype == HGEMM_DTYPE_F32 ? 4 : 2;
-    if (hgw::misaligned(y, size)) return HGEMM_ERR_ALIGNMENT;
-    const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    int sms = 0, dev = 0;
-    if (K == 0) {
-        if (int rc = hgw::current_device(&sms, &dev)) return rc;
-        const size_t bytes = static_cast<size_t>(M) * N * size;
-        return cudaMemsetAsync(y, 0, bytes, s) == cudaSuccess ? HGEMM_OK : HGEMM_ERR_CUDA;
-    }
-    if (!x) return HGEMM_ERR_INVALID_VALUE;
-    if (int rc = hgw::check_weight(q, scales, zeros, 16)) return rc;
-    if (hgw::misaligned(x, size)) return HGEMM_ERR_ALIGNMENT;
-    if (int rc = hgw::current_device(&sms, &dev)) return rc;
-    if (M > 65535 * 8) return HGEMM_ERR_UNSUPPORTED;  // grid.y
-    hgw::LinearParams p{x, M > 1 ? ldx : 0, y, M, N, K, hgw::make_weight(q, scales, zeros, N, K, group),
-                        !hgw::misaligned(x, 16) && K % 8 == 0 && (M == 1 || ldx % (16 / size) == 0)};
-    return hgw::with_format(group, zeros != nullptr, [&](auto g, auto z) {
-        constexpr int G = decltype(g)::value;
-        constexpr bool Z = decltype(z)::value;
-        return x_dtype == HGEMM_DTYPE_F32 ? hgw::run_linear<float, G, Z>(p, sms, dev, s)
-                                          : hgw::run_linear<__nv_bfloat16, G, Z>(p, sms, dev, s);
-    });
+    return gemm_w4(x, x_dtype, ldx, q, scales, zeros, y, M, N, K, group, false, stream);
+}
+
+int hgemm_debug_stalled_w4(const void* x, long long ldx, const void* q, const void* scales, const void* zeros, void* y,
+                           int M, int N, int K, int group, hgemm_stream_t stream) {
+    // The kernel with bounded waits takes more than 16 rows of aligned bf16 x.
+    if (M <= 16 || K <= 0 || K % 8 || ldx % 8 || hgw::misaligned(x, 16)) return HGEMM_ERR_INVALID_VALUE;
+    return gemm_w4(x, HGEMM_DTYPE_BF16, ldx, q, scales, zeros, y, M, N, K, group, true, stream);
 }
 
 }  // extern "C"

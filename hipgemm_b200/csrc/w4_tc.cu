@@ -38,9 +38,9 @@ static int launch_tc(const TcParams& p, int sms, int dev, cudaStream_t stream) {
 }
 
 // x: rows 16-byte aligned, K a multiple of 8.
-int run_tc(const void* x, long long ldx, void* y, int M, int N, int K, const Weight& w, int group, int sms, int dev,
-           cudaStream_t stream) {
-    TcParams p{static_cast<const __nv_bfloat16*>(x), ldx, static_cast<__nv_bfloat16*>(y), M, N, K, w, hg::status_word(dev)};
+int run_tc(const void* x, long long ldx, void* y, int M, int N, int K, const Weight& w, int group, bool stall, int sms,
+           int dev, cudaStream_t stream) {
+    TcParams p{static_cast<const __nv_bfloat16*>(x), ldx, static_cast<__nv_bfloat16*>(y), M, N, K, w, hg::status_word(dev), stall};
     if (!p.status) return HGEMM_ERR_CUDA;
     return with_format(group, w.zeros != nullptr, [&](auto g, auto z) {
         constexpr int G = decltype(g)::value;

@@ -37,6 +37,7 @@ struct TcParams {
     int M, N, K;
     Weight w;
     uint32_t* status;
+    bool stall;  // test hook (hgemm_debug_stalled_w4 only): the first step's x is never reported as copied
 };
 
 constexpr int kCopyWarps = 3;
@@ -342,7 +343,7 @@ __global__ void __launch_bounds__(TcShape<NC>::kWarps * 32, 1) w4_tc_kernel(cons
             copy_wait<S::kXAhead>();
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the MMA reads through the async proxy
             __syncwarp();
-            if (lane == 0) hg::mbar_arrive(bar(bars.full[static_cast<uint32_t>(s) % S::kAStages]));
+            if (lane == 0 && !(p.stall && s == 0)) hg::mbar_arrive(bar(bars.full[static_cast<uint32_t>(s) % S::kAStages]));
         }
         copy_wait<0>();
     } else {

@@ -316,6 +316,12 @@ int hgemm_dequantize_w4(const void* q, const void* scales, const void* zeros, in
 int hgemm_w4_gemm_tn(const void* x, int x_dtype, long long ldx, const void* q, const void* scales, const void* zeros,
                      void* y, int M, int N, int K, int group, hgemm_stream_t stream);
 
+/* Test hook for the failure path, as hgemm_debug_stalled_gemm: the product of more than 16 aligned
+ * bf16 rows (K % 8 == 0), whose kernel is never told that the first step of x is there, so that its
+ * bounded waits expire (about 2 s); it records a status, drains and returns, y is unspecified. */
+int hgemm_debug_stalled_w4(const void* x, long long ldx, const void* q, const void* scales, const void* zeros, void* y,
+                           int M, int N, int K, int group, hgemm_stream_t stream);
+
 /* ---- mixture of experts ----------------------------------------------------------------------- */
 
 /* The router of a mixture of experts: logits = x[T x D] . router[E x D]^T (both of x_dtype),
