@@ -125,8 +125,12 @@ _nothing = _Nothing()
 
 def _context(dev: int, stream: torch.cuda.Stream | None):
     """A context for a call on `dev` and `stream`; none where both are current already."""
-    if stream is None and _get_device is not None and _get_device() == dev:
-        return _nothing
+    if stream is None:
+        if _get_device is not None and _get_device() == dev:
+            return _nothing
+    elif stream.device_index != dev:
+        # The kernel would run there, on pointers into another device's memory.
+        raise ValueError(f"stream is on cuda:{stream.device_index}, the tensors are on cuda:{dev}")
     return _on(dev, stream)
 
 
