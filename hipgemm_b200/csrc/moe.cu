@@ -600,6 +600,10 @@ int hgemm_w4_moe(const void* x, int x_dtype, long long ldx, const int* ids, cons
     }
     if (!workspace || workspace_bytes < hgemm_w4_moe_workspace_bytes(T, top_k, D, F)) return HGEMM_ERR_INVALID_VALUE;
     if (hgw::misaligned(workspace, 16)) return HGEMM_ERR_ALIGNMENT;
+    // A launch's out is written when its x has been read, but before the next launch's x is: out may be x itself, whose
+    // rows end before those of the next launch's begin.
+    if (T > hgw::tokens_per_launch(top_k) && out != x && hgw::meets_rows(out, static_cast<size_t>(T) * D * size, x, T, ldx, D, size))
+        return HGEMM_ERR_INVALID_VALUE;
     if (int rc = hgw::current_device(&sms, &dev)) return rc;
 
     const int most = hgw::tokens_per_launch(top_k);

@@ -817,6 +817,8 @@ int gemm_w4(const void* x, int x_dtype, long long ldx, const void* q, const void
     if (!x) return HGEMM_ERR_INVALID_VALUE;
     if (int rc = hgw::check_weight(q, scales, zeros, 16)) return rc;
     if (hgw::misaligned(x, size)) return HGEMM_ERR_ALIGNMENT;
+    // CTAs read x while others write y.
+    if (hgw::meets_rows(y, static_cast<size_t>(M) * N * size, x, M, ldx, K, size)) return HGEMM_ERR_INVALID_VALUE;
     if (int rc = hgw::current_device(&sms, &dev)) return rc;
     if (M > 65535 * 8) return HGEMM_ERR_UNSUPPORTED;  // grid.y
     hgw::LinearParams p{x, M > 1 ? ldx : 0, y, M, N, K, hgw::make_weight(q, scales, zeros, N, K, group),

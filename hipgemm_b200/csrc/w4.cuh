@@ -855,6 +855,16 @@ int launch(dim3 grid, int threads, int cluster, size_t smem, cudaStream_t stream
 
 inline bool misaligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1u)) != 0; }
 
+// Whether `y_bytes` from y on meet one of `rows` rows of x, `ld` apart, of `columns` elements of `size` bytes.
+inline bool meets_rows(const void* y, size_t y_bytes, const void* x, int rows, long long ld, int columns, unsigned size) {
+    const uintptr_t x0 = reinterpret_cast<uintptr_t>(x), y0 = reinterpret_cast<uintptr_t>(y);
+    const size_t row = static_cast<size_t>(columns) * size, step = rows > 1 ? static_cast<size_t>(ld) * size : row;
+    if (rows < 1 || row == 0 || y_bytes == 0 || y0 >= x0 + (rows - 1) * step + row) return false;
+    if (y0 < x0) return x0 - y0 < y_bytes;
+    const size_t r = (y0 - x0) / step, at = (y0 - x0) % step;  // y starts in row r, or behind it
+    return at < row || (r + 1 < static_cast<size_t>(rows) && at + y_bytes > step);
+}
+
 // Calls go(std::integral_constant<int, GROUP>, std::bool_constant<ZERO>) for a weight's group size and kind.
 template <typename Go>
 int with_format(int group, bool zeros, Go go) {

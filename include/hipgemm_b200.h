@@ -311,7 +311,7 @@ int hgemm_dequantize_w4(const void* q, const void* scales, const void* zeros, in
  * long.)  Any N and K, M <= 524280 (HGEMM_ERR_UNSUPPORTED above); y is fully
  * overwritten; K == 0 writes zeros.  W is read once per 8 rows of fp32 or 16 to 64 of bf16 x, so
  * for many rows dequantise it instead.  The result's bits depend on the inputs alone.  Needs no
- * workspace.  x, y aligned to their element.  The first call on a device, outside any stream
+ * workspace.  x, y aligned to their element, y apart from x (HGEMM_ERR_INVALID_VALUE).  The first call on a device, outside any stream
  * capture, as for the GEMM. */
 int hgemm_w4_gemm_tn(const void* x, int x_dtype, long long ldx, const void* q, const void* scales, const void* zeros,
                      void* y, int M, int N, int K, int group, hgemm_stream_t stream);
@@ -351,6 +351,8 @@ typedef struct {
  * product between the matrices is kept in fp32.  Codes of an expert are
  * read once per 8 or 16 of its tokens; tokens beyond 64 (or 512 / top_k) take further launches.  The
  * result's bits depend on the inputs alone.
+ * out may be x; otherwise, beyond the tokens of one launch, it has to be apart from x
+ * (HGEMM_ERR_INVALID_VALUE).
  * workspace: device memory, 16-byte aligned, hgemm_w4_moe_workspace_bytes(); its content does not
  * matter.  Calls that share one must not overlap on the GPU.  E <= 1024 and top_k <= 16, else
  * HGEMM_ERR_UNSUPPORTED. */

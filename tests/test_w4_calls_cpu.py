@@ -1,4 +1,5 @@
 """Calls of the 4-bit weight operators that are refused before anything is launched."""
+import ctypes
 import types
 
 import pytest
@@ -22,3 +23,28 @@ def test_a_stream_of_another_device_is_refused():
     """Every operator enters this context before it allocates or launches anything."""
     with pytest.raises(ValueError, match="stream is on cuda:1, the tensors are on cuda:0"):
         w4._context(0, types.SimpleNamespace(device_index=1, device_type=1, stream_id=0))
+
+
+# x has 4 rows of 64 bf16, 80 apart; y 4 rows of 16: 128 bytes.  (Outputs that are not refused: test_w4_calls_gpu.py.)
+@pytest.mark.parametrize("at", [0, 2, 126, 128, -126, 160, 3 * 160, 3 * 160 + 126])
+def test_product_into_its_own_operand_is_refused(at):
+    """CTAs would read what others have written."""
+    assert hg.lib().hgemm_w4_gemm_tn(FAKE, 1, 80, FAKE * 16, FAKE * 32, None, FAKE + at, 4, 16, 64, 64, None) == INVALID
+
+
+def test_product_into_a_gap_that_is_too_small_is_refused():
+    for at, n in [(128, 9), (130, 8), (126, 8)]:  # the gap is 32 bytes, y two rows of n
+        assert hg.lib().hgemm_w4_gemm_tn(FAKE, 1, 80, FAKE * 16, FAKE * 32, None, FAKE + at, 2, n, 64, 64, None) == INVALID
+
+
+class _Weight(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("zeros", ctypes.c_void_p), ("group", ctypes.c_int)]
+
+
+@pytest.mark.parametrize("t,at", [(65, 2), (65, -2), (100, 64 * 128), (100, -64 * 128)])
+def test_experts_of_several_launches_into_their_own_operand_are_refused(t, at):
+    """Rows of x that a later launch reads would have been written by an earlier one."""
+    weight = _Weight(FAKE * 16, FAKE * 32, None, 64)
+    w, x = ctypes.addressof(weight), FAKE * 4
+    assert hg.lib().hgemm_w4_moe(x, 1, 64, FAKE * 48, FAKE * 49, t, 2, 8, 64, 32, w, w, w, x + at, FAKE * 50, 1 << 24,
+                                 None) == INVALID
