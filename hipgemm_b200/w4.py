@@ -8,7 +8,8 @@ over them (a few tokens at a time: decoding).
 
 The buffers' layout is in include/hipgemm_b200.h; the reference (nirw4nna/hipgemm) has no
 counterpart.  Every function works on the tensors' device, on `stream` or torch's current one,
-and can be captured into a CUDA graph after one call on the device.
+and can be captured into a CUDA graph after one call on the device.  Inference only: the products,
+the router and the experts refuse operands that require a gradient unless gradients are off.
 """
 from __future__ import annotations
 
@@ -93,6 +94,15 @@ def _check_rows(name: str, x: torch.Tensor) -> tuple[int, int, int]:
         raise ValueError(f"{name} must be a 2-D tensor with contiguous, non-overlapping rows")
     dt = _DTYPES.get(x.dtype)
     return ld, _dtype_code(name, x) if dt is None else dt, dev
+
+
+def _check_no_gradient(**tensors: torch.Tensor) -> None:
+    """These operators have no backward pass: a result that is cut off from its operands must not look like one
+    that is not."""
+    if torch.is_grad_enabled():
+        for name, t in tensors.items():
+            if t.requires_grad:
+                raise ValueError(f"{name} requires a gradient, which this operator does not give: detach it, or call under torch.no_grad()")
 
 
 class _on:
@@ -212,6 +222,8 @@ def w4_gemm_tn(x: torch.Tensor, w: W4Weight, out: torch.Tensor | None = None, *,
                stream: torch.cuda.Stream | None = None) -> torch.Tensor:
     """y[M,N] = x[M,K] @ W[N,K]^T for a few rows of x (fp32 or bf16, rows may be strided); y has x's
     type, sums are fp32 (hgemm_w4_gemm_tn).  For many rows use dequantize_w4 and a matrix product."""
+    if x.requires_grad:
+        _check_no_gradient(x=x)
     ldx, dt, dev = _check_rows("x", x)
     _check_weight("w", w, dev, None)
     m, k = x.shape
@@ -235,6 +247,8 @@ def moe_route(x: torch.Tensor, router: torch.Tensor, top_k: int, *, renormalize:
     """The router of a mixture of experts (hgemm_moe_route): softmax(x[T,D] @ router[E,D]^T) and per
     token the top_k largest: ids (T, top_k) int32, largest first, and their probabilities (T,
     top_k) float32, which add up to 1 with renormalize.  E <= 1024, top_k <= 16."""
+    if x.requires_grad or router.requires_grad:
+        _check_no_gradient(x=x, router=router)
     ldx, dt, dev = _check_rows("x", x)
     if router.dtype != x.dtype or router.dim() != 2 or not router.is_contiguous() or router.get_device() != dev:
         raise ValueError("router must be a contiguous (E, D) tensor of x's type on x's device")
@@ -261,6 +275,8 @@ def w4_moe(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate: W4We
     them (ids outside [0, E) add nothing), gate and up (E, F, D), down (E, D, F).  workspace:
     hgemm_w4_moe_workspace_bytes(T, top_k, D, F) bytes that no other running call uses, else
     allocated by torch."""
+    if x.requires_grad or weights.requires_grad:
+        _check_no_gradient(x=x, weights=weights)
     ldx, dt, dev = _check_rows("x", x)
     t, d = x.shape
     e, f = gate.experts, gate.n

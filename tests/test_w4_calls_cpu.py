@@ -3,6 +3,7 @@ import ctypes
 import types
 
 import pytest
+import torch
 
 import hipgemm_b200 as hg
 from hipgemm_b200 import w4
@@ -48,3 +49,20 @@ def test_experts_of_several_launches_into_their_own_operand_are_refused(t, at):
     w, x = ctypes.addressof(weight), FAKE * 4
     assert hg.lib().hgemm_w4_moe(x, 1, 64, FAKE * 48, FAKE * 49, t, 2, 8, 64, 32, w, w, w, x + at, FAKE * 50, 1 << 24,
                                  None) == INVALID
+
+
+def test_operands_that_require_a_gradient_are_refused():
+    """There is no backward pass, and a detached result would look like a constant."""
+    w = hg.w4_pack(torch.zeros(32, 64, dtype=torch.uint8), torch.ones(32, 1), group=64)
+    e = hg.w4_pack(torch.zeros(4, 32, 64, dtype=torch.uint8), torch.ones(4, 32, 1), group=64)
+    x, ids, weights = torch.zeros(2, 64), torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, 1)
+    xg, wg = x.clone().requires_grad_(), weights.clone().requires_grad_()
+    calls = {"x": [lambda: hg.w4_gemm_tn(xg, w), lambda: hg.moe_route(xg, x, 1), lambda: hg.w4_moe(xg, ids, weights, e, e, e)],
+             "router": [lambda: hg.moe_route(x, xg, 1)], "weights": [lambda: hg.w4_moe(x, ids, wg, e, e, e)]}
+    for name, some in calls.items():
+        for call in some:
+            with pytest.raises(ValueError, match=f"{name} requires a gradient"):
+                call()
+            for off in (torch.no_grad(), torch.inference_mode()):
+                with off, pytest.raises(ValueError, match="CUDA"):  # the next check: there is no GPU tensor here
+                    call()
