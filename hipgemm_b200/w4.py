@@ -55,12 +55,14 @@ def _check_weight(name: str, w: W4Weight, dev: int, count: int | None) -> None:
     # product); anything else takes the detailed ones, which raise the specific error.
     q, s, z, n, k, group = w
     if group in _GROUPS:
-        rb = (1 if count is None else count) * ((n + 15) // 16)
-        groups = rb * ((k + group - 1) // group) * 16
-        if (q.numel() == rb * ((k + 63) // 64) * 512 and s.numel() == groups and q.dtype is torch.uint8
-                and s.dtype is torch.bfloat16 and q.is_contiguous() and s.is_contiguous() and q.get_device() == dev >= 0
-                and s.get_device() == dev and (z is None or (z.numel() == groups and z.dtype is torch.uint8
-                                                             and z.is_contiguous() and z.get_device() == dev))):
+        rb = (n + 15) // 16
+        if count is None:
+            blocks, groups = (rb, (k + 63) // 64, 512), (rb, (k + group - 1) // group, 8, 2)
+        else:
+            blocks, groups = (count, rb, (k + 63) // 64, 512), (count, rb, (k + group - 1) // group, 8, 2)
+        if (q.shape == blocks and s.shape == groups and q.dtype is torch.uint8 and s.dtype is torch.bfloat16
+                and q.is_contiguous() and s.is_contiguous() and q.get_device() == dev >= 0 and s.get_device() == dev
+                and (z is None or (z.shape == groups and z.dtype is torch.uint8 and z.is_contiguous() and z.get_device() == dev))):
             return
     _check_weight_in_detail(name, w, dev, count)
 

@@ -66,3 +66,32 @@ def test_operands_that_require_a_gradient_are_refused():
             for off in (torch.no_grad(), torch.inference_mode()):
                 with off, pytest.raises(ValueError, match="CUDA"):  # the next check: there is no GPU tensor here
                     call()
+
+
+class _Fake:
+    """What the wrapper's checks look at of a CUDA tensor."""
+
+    def __init__(self, shape, dtype, stride=None):
+        self.shape, self.dtype, self._stride = torch.Size(shape), dtype, stride
+        self.dim, self.numel = lambda: len(shape), lambda: self.shape.numel()
+        self.stride, self.get_device, self.is_contiguous = lambda: stride, lambda: 0, lambda: True
+
+
+def _fake_weight(n, k, group=64, lead=(), q=None, scales=None, zeros=None):
+    rb = -(-n // 16)
+    return hg.W4Weight(_Fake(q or (*lead, rb, -(-k // 64), 512), torch.uint8),
+                       _Fake(scales or (*lead, rb, -(-k // group), 8, 2), torch.bfloat16),
+                       None if zeros is None else _Fake(zeros, torch.uint8), n, k, group)
+
+
+def test_buffers_of_another_shape_with_as_many_elements_are_refused():
+    w4._check_weight("w", _fake_weight(40, 200), 0, None)
+    w4._check_weight("w", _fake_weight(40, 200, lead=(5,), zeros=(5, 3, 4, 8, 2)), 0, 5)
+    for part, weight, count in [("q", _fake_weight(40, 200, q=(4, 3, 512)), None), ("q", _fake_weight(40, 200, q=(3, 512, 4)), None),
+                                ("q", _fake_weight(40, 200, q=(1, 3, 4, 512)), None), ("scales", _fake_weight(40, 200, scales=(4, 3, 8, 2)), None),
+                                ("scales", _fake_weight(40, 200, scales=(3, 4, 2, 8)), None),
+                                ("zeros", _fake_weight(40, 200, zeros=(4, 3, 8, 2)), None),
+                                ("q", _fake_weight(40, 200, lead=(5,), q=(3, 5, 4, 512)), 5),
+                                ("scales", _fake_weight(40, 200, lead=(5,), scales=(15, 4, 8, 2)), 5)]:
+        with pytest.raises(ValueError, match=rf"w\.{part} must be"):
+            w4._check_weight("w", weight, 0, count)
