@@ -23,6 +23,7 @@ from .gemm import _fn, _get_device, _stream_handle
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 _GROUPS = (32, 64, 128)
+_MOST = 2 ** 31 - 1  # the C functions' sizes are ints, and ctypes cuts larger ones off without a word
 
 
 class W4Weight(NamedTuple):
@@ -54,7 +55,7 @@ def _check_weight(name: str, w: W4Weight, dev: int, count: int | None) -> None:
     # A few cheap tests in the common case (this wrapper's host time adds to every launch of a small
     # product); anything else takes the detailed ones, which raise the specific error.
     q, s, z, n, k, group = w
-    if group in _GROUPS:
+    if group in _GROUPS and 0 <= n <= _MOST and 0 <= k <= _MOST:
         rb = (n + 15) // 16
         if count is None:
             blocks, groups = (rb, (k + 63) // 64, 512), (rb, (k + group - 1) // group, 8, 2)
@@ -71,6 +72,8 @@ def _check_weight_in_detail(name: str, w: W4Weight, dev: int, count: int | None)
     q, s, z, n, k, group = w
     if group not in _GROUPS:
         raise ValueError(f"{name}.group must be 32, 64 or 128, got {group}")
+    if not 0 <= n <= _MOST or not 0 <= k <= _MOST:
+        raise ValueError(f"{name} is {n} x {k}: sizes have to be below 2^31")
     rb, lead = -(-n // 16), () if count is None else (count,)
     shape = (*lead, rb, -(-k // 64), 512)
     if q.dtype != torch.uint8 or q.shape != shape or not q.is_contiguous():
@@ -92,6 +95,8 @@ def _check_rows(name: str, x: torch.Tensor) -> tuple[int, int, int]:
         raise ValueError(f"{name} must be a 2-D tensor with contiguous, non-overlapping rows")
     ld, one = x.stride()
     rows, columns = x.shape
+    if rows > _MOST or columns > _MOST:
+        raise ValueError(f"{name} is {rows} x {columns}: sizes have to be below 2^31")
     if (columns > 1 and one != 1) or (rows > 1 and ld < columns):
         raise ValueError(f"{name} must be a 2-D tensor with contiguous, non-overlapping rows")
     dt = _DTYPES.get(x.dtype)
@@ -188,6 +193,8 @@ def quantize_w4(w: torch.Tensor, group: int = 128, zero_point: bool = False,
     if group not in _GROUPS:
         raise ValueError(f"group must be 32, 64 or 128, got {group}")
     *lead, n, k = w.shape
+    if max(w.shape) > _MOST:
+        raise ValueError(f"w is {tuple(w.shape)}: sizes have to be below 2^31")
     rb, dev = -(-n // 16), w.get_device()
     with _context(dev, stream):
         q = w.new_empty((*lead, rb, -(-k // 64), 512), dtype=torch.uint8)
@@ -256,6 +263,8 @@ def moe_route(x: torch.Tensor, router: torch.Tensor, top_k: int, *, renormalize:
         raise ValueError("router must be a contiguous (E, D) tensor of x's type on x's device")
     t, d = x.shape
     e = router.shape[0]
+    if top_k > _MOST:
+        raise ValueError("top_k has to be below 2^31")
     if router.shape[1] != d:
         raise ValueError(f"D mismatch: x is {tuple(x.shape)}, router is {tuple(router.shape)}")
     with _context(dev, stream):

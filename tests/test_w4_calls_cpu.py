@@ -95,3 +95,14 @@ def test_buffers_of_another_shape_with_as_many_elements_are_refused():
                                 ("scales", _fake_weight(40, 200, lead=(5,), scales=(15, 4, 8, 2)), 5)]:
         with pytest.raises(ValueError, match=rf"w\.{part} must be"):
             w4._check_weight("w", weight, 0, count)
+
+
+def test_sizes_that_do_not_fit_an_int_are_refused():
+    """They would be cut off on the way to the library: 2^32 + 64 columns would be 64."""
+    for n, k in [(40, 2 ** 32 + 64), (2 ** 32 + 40, 64), (40, 2 ** 31), (-16, 64)]:
+        with pytest.raises(ValueError, match="2\\^31"):
+            w4._check_weight("w", _fake_weight(n, k), 0, None)
+    for shape in [(2 ** 31, 64), (2, 2 ** 32 + 64)]:
+        with pytest.raises(ValueError, match="2\\^31"):
+            w4._check_rows("x", _Fake(shape, torch.bfloat16, (shape[1], 1)))
+    assert w4._check_rows("x", _Fake((2 ** 31 - 1, 64), torch.bfloat16, (64, 1))) == (64, 1, 0)
