@@ -776,9 +776,10 @@ int run_linear(const LinearParams& p, int sms, int dev, cudaStream_t stream) {
         // 34.3, 7168 x 2048 4.5 and 5.6, 4096 x 1024 3.9 and 2.8).  Three to eight rows take three times the integer
         // instructions: 8192 x 8192 16.5 and 12.7.
         if (p.M <= 2 && run_rows<T, 0, GROUP, ZERO>(p, 6, sms, dev, stream, &rc)) return rc;
-        // The tensor cores from 17 rows on (us below and there, at 8192 x 8192 and at 28672 x 8192): 16 rows 14.8 and 14.5,
-        // 46.4 and 43.2, but 5.6 and 7.4 at 4096 x 4096; 17 rows 28.5 and 16.7, 86.4 and 51.7; 64 rows 44.3 and
-        // 21.7, 153 and 68.2.
+        // The tensor cores from 17 rows on (us below and there, groups of 128, at 4096 x 4096, 8192 x 8192 and 28672 x 8192):
+        // 9 rows 5.6 and 7.6, 15.1 and 16.6, 45.5 and 51.3; 16 rows 5.8 and 7.7, 15.4 and 16.9, 47.0 and 52.3 (8192 x
+        // 8192 in groups of 64 20.0 and 18.0, of 32 with zero points 23.6 and 25.5); 17 rows, of the last two, 28.5 and
+        // 16.9, 86.4 and 51.7; 64 rows 44.3 and 22.1, 153 and 68.2.
         if (p.M > 16 && p.vec) return run_tc(p.x, p.ldx, p.y, p.M, p.N, p.K, p.w, GROUP, p.stall, sms, dev, stream);
         if (p.M <= 8) return launch_linear<T, 2, 1, 3, GROUP, ZERO, 8>(p, sms, dev, stream);
         if (p.M <= 16) return launch_linear<T, 2, 2, 3, GROUP, ZERO, 4>(p, sms, dev, stream);

@@ -12,8 +12,9 @@
 // Scales and zero points: [row block][group][g][rr].
 //
 // Numerics: 128 + code is exact in bf16 (0x4300 | code), and so is its difference to 128 + zero.
-// Products of two bf16 are exact, the tensor core sums a 32- or 64-deep part of a group in
-// fp32, and the scale multiplies that sum in fp32: nothing is rounded to 16 bits on the way.
+// Products of two bf16 are exact, the tensor core sums a whole group (32, 64 or 128 K) in fp32, and
+// the scale multiplies that sum in fp32: nothing is rounded to 16 bits on the way.  A group's sum
+// has no scale in it yet: 128 products of 15 x leave fp32's range from |x| = 2^117 on.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -831,7 +832,9 @@ int resident_ctas(int dev, int threads, size_t bytes) {
 }
 
 // Launches KERNEL with a cluster of `cluster` CTAs.  Programmatic dependent launch: the CTAs may start while the
-// stream's previous kernel ends; they touch global memory only after griddepcontrol.wait.
+// stream's previous kernel ends; they touch global memory only after griddepcontrol.wait, but for ids and weights of
+// the experts, which their second and third kernel read before it: the first waits before it triggers, so that
+// whatever wrote those has ended when the others start.
 template <auto KERNEL, typename... Args>
 int launch(dim3 grid, int threads, int cluster, size_t smem, cudaStream_t stream, const Args&... args) {
     cudaLaunchConfig_t cfg{};

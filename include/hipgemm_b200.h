@@ -308,9 +308,11 @@ int hgemm_dequantize_w4(const void* q, const void* scales, const void* zeros, in
  * in full, except that an element of fp32 x may be held to 2^-20 of itself, whatever lies beside
  * it.  (One or two rows, and rows of fp32, are held as whole numbers; where elements of up to 512
  * consecutive K lie more than about 2^24 (bf16) or 2^19 (fp32) apart, the call takes up to twice as
- * long.)  Any N and K, M <= 524280 (HGEMM_ERR_UNSUPPORTED above); y is fully
- * overwritten; K == 0 writes zeros.  W is read once per 8 rows of fp32 or 16 to 64 of bf16 x, so
- * for many rows dequantise it instead.  The result's bits depend on the inputs alone.  Needs no
+ * long.)  A group's sum of (code - zero) x is formed before it is scaled: elements of 2^117 and
+ * above can make it an infinity where the scaled sum is none.  Any N and K, M <= 524280 (HGEMM_ERR_UNSUPPORTED above); y is fully
+ * overwritten; K == 0 writes zeros.  W is read once per 8 rows of fp32 or 16 to 64 of bf16 x: from
+ * about 16 rows of a large W on, FP8 is faster (hgemm_fp8_tn), from 64 on W dequantised and any
+ * product of bf16.  The result's bits depend on the inputs alone.  Needs no
  * workspace.  x, y aligned to their element, y apart from x (HGEMM_ERR_INVALID_VALUE).  The first call on a device, outside any stream
  * capture, as for the GEMM. */
 int hgemm_w4_gemm_tn(const void* x, int x_dtype, long long ldx, const void* q, const void* scales, const void* zeros,
@@ -347,8 +349,8 @@ typedef struct {
  * x: T x D fp32 or bf16, `ldx` elements from row to row; out: T x D row-major of the same type;
  * gate and up: stacks of E (F x D) of the same group size, both with or both without zero
  * points; down: a stack of E (D x F).  An id outside [0, E) adds nothing (padding, experts of
- * another rank); an id that a token has twice counts with both weights.  Sums in fp32; the
- * product between the matrices is kept in fp32.  Codes of an expert are
+ * another rank); an id that a token has twice counts with both weights.  Sums in fp32, with the
+ * range of hgemm_w4_gemm_tn; the product between the matrices is kept in fp32.  Codes of an expert are
  * read once per 8 or 16 of its tokens; tokens beyond 64 (or 512 / top_k) take further launches.  The
  * result's bits depend on the inputs alone.
  * out may be x; otherwise, beyond the tokens of one launch, it has to be apart from x

@@ -122,3 +122,26 @@ def test_weights_that_meet_the_small_elements_alone(cuda_device, m, n, k, group,
     codes = torch.where(large, none, codes)
     w = hg.w4_pack(codes.cuda(), scales.cuda(), None if zeros is None else zeros.cuda(), group=group)
     ref.assert_close(hg.w4_gemm_tn(x.cuda(), w), *ref.linear(x, ref.values(codes, scales, zeros, group), TERMS[dtype]), dtype)
+
+
+# ---- range ----------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("m,dtype", [*ROWS, (5, torch.bfloat16), (12, torch.bfloat16), (40, torch.bfloat16), (70, torch.bfloat16)])
+@pytest.mark.parametrize("n,k,group", [(5120, 1024, 128), (50, 256, 64), (4097, 1100, 32)])
+def test_elements_up_to_the_documented_range(cuda_device, m, dtype, n, k, group):
+    """Every code 15 steps from its zero point and every element just below 2^117, against a scale that brings the result
+    back: no sum on the way is an infinity."""
+    sign = (torch.arange(k) // group % 2 * 2 - 1).float()  # groups alternate: their scaled sums nearly cancel
+    codes = torch.full((n, k), 15, dtype=torch.uint8)
+    scales = torch.full((n, -(-k // group)), 2.0 ** -20)
+    zeros = torch.zeros(n, -(-k // group), dtype=torch.uint8)
+    w = hg.w4_pack(codes.cuda(), scales.cuda(), zeros.cuda(), group=group)
+    x = (sign * 2.0 ** 117 * (1 - 2.0 ** -8)).expand(m, k).to(dtype)
+    got = hg.w4_gemm_tn(x.cuda(), w)
+    assert bool(got.isfinite().all())
+    ref.assert_close(got, *ref.linear(x, ref.values(codes, scales, zeros, group), TERMS[dtype]), dtype)
+    # Beyond it an infinity is one that the products' true sum leads to, never a NaN or a wrong number.
+    got = hg.w4_gemm_tn((x.abs().double() * 4).to(dtype).cuda(), w).cpu()
+    want = float(x.abs()[0, 0]) * 4 * 15 * 2.0 ** -20 * k
+    assert bool(((got == float("inf")) | ((got.double() - want).abs() <= want * 2.0 ** -7)).all())
