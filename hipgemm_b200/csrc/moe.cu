@@ -516,11 +516,11 @@ int launch_experts(const ExpertParams& p, int sms, int dev, cudaStream_t stream)
     return launch<kernel>(dim3(static_cast<unsigned>(most < wave ? most : wave)), kMoeThreads, 1, Shape::kSmem, stream, p);
 }
 
-// WK: 2 where that gives units enough, else 4.  Measured (bf16, groups of 128; WK = 2, 4, 8): 32 tokens through 6 of 64
-// experts of 4096 x 2048, gate and up 145, 148, 156 us, down 92, 102, 110; 4 tokens through 8 of 64 of
-// 2048 x 1024, 19.0, 20.9, 21.9 and 14.5, 12.5, 13.4; one token 10.2, 10.5, 9.6 and 7.3, 5.3, 5.4.  Two row
-// blocks of down (4 of gate and up) a warp: 120 us with one for down, but 177 instead of 145 for gate and
-// up, whose CTAs then fit an SM once instead of three times.
+// WK: 2 where that gives units enough, else 4.  Measured (bf16, groups of 128; WK = 2, 4, 8): gate and up of 32 tokens
+// through 6 of 64 experts of 4096 x 2048 145, 148, 156 us, of 4 tokens through 8 of 64 of 2048 x 1024 19.0,
+// 20.9, 21.9, of one token 10.2, 10.5, 9.6; the three kernels together, by down's WK, 289, 297, 302, then 49.3,
+// 46.2, 47.4, then 22.2, 18.0, 18.2.  Two row blocks of down a warp: 347 instead of 289 with one.  But one of gate
+// and one of up: 177 instead of 145 with two, whose CTAs then fit an SM once instead of three times.
 template <typename T, int MATS, int NT, int GROUP, bool ZERO>
 int run_experts(const ExpertParams& p, int sms, int dev, cudaStream_t stream) {
     constexpr int RH = MATS == 2 ? 1 : 2;

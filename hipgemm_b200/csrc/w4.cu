@@ -708,8 +708,8 @@ int resident_clusters(int split, int sms, int dev) {
 }
 
 // Candidate `split`, for warps that may hold up to `most` steps.  The cost is a warp's steps from begin to end, two
-// for each step of x that it turns into planes, and one for the exchange between CTAs (8192 x 8192 by one row: 13.5
-// us for 1 CTA, 11.4 for 2 and 12.7 for 4; 28672 x 8192: 27.0, 25.6, 33).
+// for each step of x that it turns into planes, and one for the exchange between CTAs (8192 x 8192 by one row: 13.0
+// us for 1 CTA, 10.8 for 2 and 12.9 for 4; 28672 x 8192: 25.3, 24.8, 33).
 inline RowsPlan rows_plan(int row_blocks, int steps, int split, int clusters, int warps, int most) {
     RowsPlan plan;
     int held = ceil_div(steps, split * warps);
