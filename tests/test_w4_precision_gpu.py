@@ -145,3 +145,25 @@ def test_elements_up_to_the_documented_range(cuda_device, m, dtype, n, k, group)
     got = hg.w4_gemm_tn((x.abs().double() * 4).to(dtype).cuda(), w).cpu()
     want = float(x.abs()[0, 0]) * 4 * 15 * 2.0 ** -20 * k
     assert bool(((got == float("inf")) | ((got.double() - want).abs() <= want * 2.0 ** -7)).all())
+
+
+# ---- sums of fp32 rows ------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("m", [1, 3, 8, 20])
+@pytest.mark.parametrize("group,zero_point", [(32, True), (64, False), (64, True), (128, False), (128, True)])
+def test_one_group_of_fp32_is_rounded_twice(cuda_device, m, group, zero_point):
+    """One group of elements in [1, 2) and steps of one sign: their first terms (8 bits, 2^-7 apart) times the steps add
+    up to less than 2^12, exact in fp32 in any order."""
+    gen = _gen(m, group)
+    n, k = 64, group
+    codes = torch.randint(8, 16, (n, k), generator=gen, dtype=torch.uint8)
+    scales = torch.rand(n, 1, generator=gen).bfloat16() + 0.5
+    zeros = torch.randint(0, 8, (n, 1), generator=gen, dtype=torch.uint8) if zero_point else None
+    w = hg.w4_pack(codes.cuda(), scales.cuda(), None if zeros is None else zeros.cuda(), group=group)
+    x = torch.rand(m, k, generator=gen) + 1
+    want = x.double() @ ref.values(codes, scales, zeros, group).T
+    # The other terms are below 2^-7 of x, in group / 8 additions; then two sums are added, and scaled: half a step each.
+    bound = want * (2 * 2.0 ** -24 + group // 8 * ref.ADD * 2.0 ** -7)
+    got = hg.w4_gemm_tn(x.cuda(), w).cpu().double()
+    assert bool(((got - want).abs() <= bound).all()), float(((got - want).abs() / bound).max())
