@@ -230,7 +230,8 @@ def dequantize_w4(w: W4Weight, dtype: torch.dtype = torch.bfloat16, out: torch.T
 def w4_gemm_tn(x: torch.Tensor, w: W4Weight, out: torch.Tensor | None = None, *,
                stream: torch.cuda.Stream | None = None) -> torch.Tensor:
     """y[M,N] = x[M,K] @ W[N,K]^T for a few rows of x (fp32 or bf16, rows may be strided); y has x's
-    type, sums are fp32 (hgemm_w4_gemm_tn).  For many rows use dequantize_w4 and a matrix product."""
+    type, sums are fp32 (hgemm_w4_gemm_tn).  out may not overlap x.  From about 16 rows of a large W
+    on fp8_gemm_tn is faster, from 64 on a bf16 product with dequantize_w4's values."""
     if x.requires_grad:
         _check_no_gradient(x=x)
     ldx, dt, dev = _check_rows("x", x)
@@ -283,9 +284,9 @@ def w4_moe(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate: W4We
     """The experts of a mixture for a few tokens (hgemm_w4_moe), in three kernels:
     out[t] = sum_j weights[t,j] * down_e(silu(gate_e x[t]) * (up_e x[t])), e = ids[t,j].
     x (T, D) fp32 or bf16, ids (T, top_k) int32 and weights (T, top_k) float32 as moe_route gives
-    them (ids outside [0, E) add nothing), gate and up (E, F, D), down (E, D, F).  workspace:
-    hgemm_w4_moe_workspace_bytes(T, top_k, D, F) bytes that no other running call uses, else
-    allocated by torch."""
+    them (ids outside [0, E) add nothing), gate and up (E, F, D), down (E, D, F).  out may be x.
+    workspace: hgemm_w4_moe_workspace_bytes(T, top_k, D, F) bytes that no other running call uses,
+    else allocated by torch."""
     if x.requires_grad or weights.requires_grad:
         _check_no_gradient(x=x, weights=weights)
     ldx, dt, dev = _check_rows("x", x)

@@ -305,8 +305,8 @@ int hgemm_dequantize_w4(const void* q, const void* scales, const void* zeros, in
 
 /* y[M x N] = x[M x K] . W[N x K]^T for few rows of x (decoding): x fp32 or bf16 with `ldx`
  * elements from row to row, y row-major of the same type, sums in fp32, one rounding.  x is used
- * in full, except that an element of fp32 x may be held to 2^-20 of itself, whatever lies beside
- * it.  (One or two rows, and rows of fp32, are held as whole numbers; where elements of up to 512
+ * in full, except that an element of fp32 x may be held to 2^-20 of itself, or to 2^-133, whatever
+ * lies beside it.  (One or two rows, and rows of fp32, are held as whole numbers; where elements of up to 512
  * consecutive K lie more than about 2^24 (bf16) or 2^19 (fp32) apart, the call takes up to twice as
  * long.)  A group's sum of (code - zero) x is formed before it is scaled: elements of 2^117 and
  * above can make it an infinity where the scaled sum is none.  Any N and K, M <= 524280 (HGEMM_ERR_UNSUPPORTED above); y is fully
