@@ -278,11 +278,14 @@ __device__ __forceinline__ int counted_id(const int* ids, int p, int top_k, int 
     return id;
 }
 
-// Fills the lists from ids (T x top_k), T * top_k <= kMaxPairs.  Within an expert pairs keep their order, and so
-// do the segments: the result's bits depend on the inputs alone.  All threads call it.
-__device__ void build_lists(PairLists& s, const int* ids, int T, int top_k, int E, int columns) {
+// Fills the lists from `given` (T x top_k ids), T * top_k <= kMaxPairs.  Within an expert pairs keep their order, and
+// so do the segments: the result's bits depend on the inputs alone.  All threads call it.  `ids`: shared memory
+// for kMaxPairs numbers, free again afterwards.
+__device__ void build_lists(PairLists& s, int* ids, const int* given, int T, int top_k, int E, int columns) {
     const int pairs = T * top_k, lane = threadIdx.x & 31;
     __shared__ int done;
+    for (int p = threadIdx.x; p < pairs; p += kMoeThreads) ids[p] = __ldcg(given + p);
+    __syncthreads();
     if (threadIdx.x < 32) {
         // Up to 32 pairs, and no expert with more than a segment: all in one warp's registers.
         bool ok = false;
@@ -395,10 +398,11 @@ __global__ void __launch_bounds__(kMoeThreads) moe_expert_kernel(const ExpertPar
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, group = warp / WK, part = warp % WK;
     const Weight& first = MATS == 2 ? p.gate : p.down;
     // The next kernels look at ids (and weights) before they wait for this one.  They start when every CTA of the product
-    // with gate and up has come to its trigger, which is after its wait: whatever made ids is complete by then.
+    // with gate and up has come to its trigger, which is after its wait: whatever made ids is complete by then, and
+    // in L2, where they load it from (an SM's L1 is only sure to be up to date after the kernel's own wait).
     if (MATS == 2) pdl_wait();
     pdl_trigger();
-    build_lists(lists, p.ids, p.T, p.top_k, p.E, 8 * NT);
+    build_lists(lists, reinterpret_cast<int*>(smem), p.ids, p.T, p.top_k, p.E, 8 * NT);
     if (MATS == 1) pdl_wait();
     const int row_blocks = first.row_blocks, chunks = ceil_div(row_blocks, RH * Shape::kGroups), units = lists.n_segments * chunks;
     const int steps = ceil_div(first.k_blocks, 2), s0 = steps * part / WK, s1 = steps * (part + 1) / WK;
@@ -462,17 +466,23 @@ constexpr int kCombineThreads = 128;
 
 template <typename T>
 __global__ void __launch_bounds__(kCombineThreads) moe_combine_kernel(const ExpertParams p) {
-    __shared__ float weight[kMaxTopK];  // 0: not counted
+    __shared__ float given[kMaxTopK], weight[kMaxTopK];  // 0: not counted
+    __shared__ int ids[kMaxTopK];
     __shared__ bool counts[kMaxTopK];
-    const int t = blockIdx.y, d = (blockIdx.x * kCombineThreads + threadIdx.x) * 4;
+    const int t = blockIdx.y, d = (blockIdx.x * kCombineThreads + threadIdx.x) * 4, slot = threadIdx.x;
     pdl_trigger();
-    if (static_cast<int>(threadIdx.x) < p.top_k) {
-        const int j = threadIdx.x, id = counted_id(p.ids, t * p.top_k + j, p.top_k, p.E);
+    if (slot < p.top_k) {  // from L2, as above
+        ids[slot] = __ldcg(p.ids + t * p.top_k + slot);
+        given[slot] = __ldcg(p.weights + t * p.top_k + slot);
+    }
+    __syncthreads();
+    if (slot < p.top_k) {
+        const int id = counted_id(ids, slot, p.top_k, p.E);
         float w = 0.0f;
-        for (int q = j; q < p.top_k; ++q)
-            if (q == j || p.ids[t * p.top_k + q] == id) w += p.weights[t * p.top_k + q];
-        weight[j] = w;
-        counts[j] = id >= 0;
+        for (int q = slot; q < p.top_k; ++q)
+            if (q == slot || ids[q] == id) w += given[q];
+        weight[slot] = w;
+        counts[slot] = id >= 0;
     }
     __syncthreads();
     pdl_wait();

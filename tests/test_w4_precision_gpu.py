@@ -112,7 +112,8 @@ def test_an_outlier_that_no_weight_meets_costs_nothing(cuda_device, m, dtype, ze
 
 
 @pytest.mark.parametrize("m,dtype", ROWS, ids=ROW_IDS)
-@pytest.mark.parametrize("n,k,group,zero_point", [(5120, 1024, 128, False), (7100, 1100, 32, True), (300, 20000, 64, False)])
+@pytest.mark.parametrize("n,k,group,zero_point", [(5120, 1024, 128, False), (7100, 1100, 32, True), (300, 20000, 64, False),
+                                                  (300, 17000, 32, True)])
 def test_weights_that_meet_the_small_elements_alone(cuda_device, m, n, k, group, zero_point, dtype):
     gen = _gen(m, n, k, 9)
     codes, scales, zeros = ref.random_weight(gen, (n, k), group, zero_point)

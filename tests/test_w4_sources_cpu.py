@@ -18,3 +18,11 @@ def test_no_non_coherent_loads(name):
     """These kernels are launched with programmatic stream serialization: the kernel before them may be writing their
     operands when they start, so that no load may take the path for data that never changes while a kernel runs."""
     assert re.findall(r"__ldg|ld\.global[.\w:]*\.nc|\btex1D|__restrict__|__restrict\b", _code(name)) == []
+
+
+def test_what_is_read_before_the_wait_comes_from_l2():
+    """The experts' second and third kernel read ids and weights before griddepcontrol.wait.  What wrote them has ended
+    (the first kernel waits before it triggers), but only L2 is sure to show it to a kernel that has not waited."""
+    code = _code("moe.cu")
+    assert re.findall(r"p\.(?:ids|weights)\s*\[[^\]]*\](?!\s*=)", code) == []
+    assert len(re.findall(r"__ldcg\((?:given|p\.ids|p\.weights) \+", code)) == 3
