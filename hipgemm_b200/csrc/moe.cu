@@ -362,7 +362,7 @@ __device__ void build_lists(PairLists& s, int* ids, const int* given, int T, int
 // h = silu(gate x) * (up x) is kept in fp32 and enters the product with down as three bf16 terms, whose sum it
 // is: nothing between the two products is rounded to fewer bits.  As two bf16 (16 bits) it cost bf16 outputs
 // their last place more often than the order of summation does (2-norm of the difference to fp32's outputs
-// 1.3e-4 to 1.6e-4, now 2e-5 to 9e-5), and 240 us instead of 289 (32 tokens), 16.3 instead of 18.0 (one).
+// 1.3e-4 to 1.6e-4, now 2e-5 to 9e-5), and took 240 us instead of 285 (32 tokens), 16.3 instead of 18.1 (one).
 
 struct ExpertParams {
     const void* x;
